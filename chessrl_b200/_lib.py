@@ -21,7 +21,7 @@ DTYPE_F16, DTYPE_F8E4M3, DTYPE_I8 = 0, 1, 2
 LAYOUT_NHWC_F32, LAYOUT_NHWC_F16, LAYOUT_NCHW_F16, LAYOUT_NCHW_F32, LAYOUT_PACKED104 = 0, 1, 2, 3, 4
 PACKED104_BYTES = 840
 MASK_NONE, MASK_BITS, MASK_ADDITIVE, MASK_FROM_RECORDS = 0, 1, 2, 3
-OUT_F32, OUT_F16 = 0, 1
+OUT_F32, OUT_F16, OUT_BF16 = 0, 1, 2
 VOCAB_NATIVE, VOCAB_RL1929 = 0, 1
 FUSE_LN_AUTO, FUSE_LN_ON, FUSE_LN_OUT, FUSE_LN_OFF = 0, 1, 2, 3
 PREC_QKV_F16, PREC_LN_F32, PREC_MISH_F32, PREC_ATTN_F32, PREC_FFN_F16, PREC_ATTN_GEMM_F16 = 1, 2, 4, 8, 16, 32
@@ -32,6 +32,7 @@ EXPORTS = [
     "crl_last_launch_count", "crl_error_detail", "crl_strerror", "crl_linear", "crl_linear_ex", "crl_vocab_move",
     "crl_vocab_mirror_index", "crl_profile", "crl_profile_read", "crl_profile_entry", "crl_forward_static", "crl_perft", "crl_fen_to_planes19", "crl_legal_mask_1929",
     "crl_playout_positions", "crl_pack_planes104", "crl_legal_masks_packed104", "crl_game_records", "crl_successors",
+    "crl_kv4_page_bytes", "crl_kv4_append", "crl_kv4_read", "crl_kv4_attention", "crl_adjust_logits",
 ]
 
 
@@ -75,6 +76,52 @@ class LinearArgs(ctypes.Structure):
         ("lno_weight", ctypes.c_void_p), ("lno_bias", ctypes.c_void_p), ("lno_x8", ctypes.c_void_p),
         ("lno_out8_scale", ctypes.c_float), ("lno_scratch", ctypes.c_void_p), ("lno_qscale", ctypes.c_void_p),
     ]
+
+
+_P, _I32, _I64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+
+class Kv4Cache(ctypes.Structure):
+    """Mirror of `crl_kv4_cache` (include/chessrl_b200.h)."""
+    _fields_ = [("pages", _P), ("num_pages", _I64), ("page_size", _I32), ("kv_heads", _I32), ("head_dim", _I32),
+                ("seqs", _I32), ("block_table", _P), ("table_stride", _I64), ("table_width", _I32)]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    """Mirror of `crl_kv4_append_args`."""
+    _fields_ = [("cache", Kv4Cache), ("dtype", _I32), ("heads", _I32), ("tokens", _I64),
+                ("q", _P), ("q_token_stride", _I64), ("q_head_stride", _I64),
+                ("k", _P), ("k_token_stride", _I64), ("k_head_stride", _I64),
+                ("v", _P), ("v_token_stride", _I64), ("v_head_stride", _I64),
+                ("q_out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+                ("starts", _P), ("cu_tokens", _P), ("rope", _P), ("rope_positions", _I64), ("rope_dim", _I32),
+                ("rope_interleaved", _I32), ("device_status", _P), ("stream", _P)]
+
+
+class Kv4ReadArgs(ctypes.Structure):
+    """Mirror of `crl_kv4_read_args`."""
+    _fields_ = [("cache", Kv4Cache), ("dtype", _I32), ("tokens", _I64),
+                ("k", _P), ("k_token_stride", _I64), ("k_head_stride", _I64),
+                ("v", _P), ("v_token_stride", _I64), ("v_head_stride", _I64),
+                ("starts", _P), ("cu_tokens", _P), ("device_status", _P), ("stream", _P)]
+
+
+class Kv4AttentionArgs(ctypes.Structure):
+    """Mirror of `crl_kv4_attention_args`."""
+    _fields_ = [("cache", Kv4Cache), ("dtype", _I32), ("heads", _I32), ("tokens", _I64),
+                ("q", _P), ("q_token_stride", _I64), ("q_head_stride", _I64),
+                ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+                ("lengths", _P), ("cu_tokens", _P), ("max_tokens", _I32), ("scale", _F32), ("device_status", _P), ("stream", _P)]
+
+
+class LogitsArgs(ctypes.Structure):
+    """Mirror of `crl_logits_args`."""
+    _fields_ = [("dtype", _I32), ("vocab", _I32), ("rows", _I64), ("in", _P), ("in_stride", _I64),
+                ("out", _P), ("out_stride", _I64), ("history", _P), ("history_stride", _I64), ("history_len", _I32),
+                ("repetition", _P), ("frequency", _P), ("presence", _P),
+                ("bias_ids", _P), ("bias_stride", _I64), ("bias_values", _P), ("value_stride", _I64), ("biases", _I32),
+                ("mask", _P), ("mask_stride", _I64), ("mask_count", _I64), ("mask_rows", _P), ("masked_value", _F32),
+                ("device_status", _P), ("stream", _P)]
 
 
 _lib = None
@@ -157,6 +204,12 @@ def load():
     lib.crl_vocab_move.restype = ctypes.c_int
     lib.crl_vocab_mirror_index.argtypes = [ctypes.c_int]
     lib.crl_vocab_mirror_index.restype = ctypes.c_int
+    lib.crl_kv4_page_bytes.argtypes = [i32, i32, i32]
+    lib.crl_kv4_page_bytes.restype = ctypes.c_size_t
+    for name, args in (("crl_kv4_append", Kv4AppendArgs), ("crl_kv4_read", Kv4ReadArgs),
+                       ("crl_kv4_attention", Kv4AttentionArgs), ("crl_adjust_logits", LogitsArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args)]
+        getattr(lib, name).restype = ctypes.c_int
     _lib = lib
     return lib
 

@@ -1,0 +1,539 @@
+// Attention of few query rows (single tokens, short runs) over the 4-bit cache of kv4.cuh.
+//
+// out = softmax(scale * q K^T) V. A sequence's new tokens are the last of its cached ones: new token j of n at length L
+// sees cache indices 0 .. L - n + j. One cluster of CTAs per (sequence, key head, tile of 8 NT query rows); its warps
+// take tiles of 64 keys in turn, each with a running maximum, sum and output of its own (fp32), joined over the CTA and
+// then over the cluster through distributed shared memory: no workspace, one launch.
+//
+// A row (token j, head h of the g that share the key head) is number j * g + h. Matrix products are
+// mma.m16n8k16 with KEYS as the 16 rows and query rows as the 8 columns: for a few rows that wastes half as much as the
+// other way round, and a lane's operand registers come straight from one aligned word of codes, see kv4.cuh:
+//   word & 0x000f000f, word & 0x00f000f0 (and the same of word >> 8) are pairs of f16 subnormals n * 2^-24, n * 2^-20:
+//   exact operands for one logical instruction per two codes. The factor 16 of every other pair is taken out of q
+//   beforehand (scores) or out of the result (output); the offset 8 is the accumulator's start (scores) or comes out
+//   of one more product with a constant operand (output).
+// Scores: S = sum over groups of s_k * (q . (n - 8)) + c_k * sum(q), exact codes, q scaled to [1, 2) per row, fp32.
+// Output: P' = p * s rounded to f16 once, relative to the largest step seen so far (a power of two R per group), times the
+// codes; the centres' share p * c is summed in fp32. The products with n and with the offset 8 share the rounded P', so
+// its rounding weighs on the centred codes only.
+//
+// Bound by memory: 20 hd bytes per 16 cached tokens and key head, brought in by one bulk copy per block into a ring that
+// belongs to the warp (no barrier among warps before the join).
+#pragma once
+#include <type_traits>
+
+#include "kv4.cuh"
+
+namespace crl {
+
+struct Kv4AttentionParams {
+  const uint8_t* pages;
+  Kv4Table table;
+  const int32_t* lengths;     // [seqs] cached tokens, the new ones included
+  const int32_t* cu;          // [seqs + 1] first query row of each sequence; null: one token each
+  int32_t seqs, kv_heads, group;   // group: query heads per key head
+  int32_t max_tokens;         // most new tokens of a sequence
+  int32_t row_tiles;
+  int64_t tokens;             // token rows of q and out
+  const void* q;
+  void* out;
+  int64_t q_tok, q_head, o_tok, o_head;
+  int32_t vec_q;
+  float scale_log2;           // softmax scale * log2(e)
+  int* status;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float cluster_ld_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {
+  if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+  else { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+}
+
+template <int HD, int NT, int WARPS, int STAGES>
+struct Kv4AttnShape {
+  static constexpr int kTile = 4;                                  // blocks of a tile
+  static constexpr int kStage = kTile * kv4_block_bytes(HD);
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kRing = WARPS * STAGES * kStage;
+  static constexpr int kPart = kRows * (HD + 2) * 4;               // a warp's output, maximum and sum
+  static constexpr int kJoin = (WARPS + 1) * kPart;                // the warps' and the CTA's
+  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + WARPS * STAGES * 8;
+};
+
+template <typename T, int HD, int NT, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4AttentionParams p) {
+  using Shape = Kv4AttnShape<HD, NT, WARPS, STAGES>;
+  constexpr int G = HD / 32, MT = HD / 16, BB = kv4_block_bytes(HD), TB = Shape::kTile, ROWS = Shape::kRows;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int head = blockIdx.y % p.kv_heads, row_tile = blockIdx.y / p.kv_heads, seq = blockIdx.z;
+  uint8_t* ring = smem + warp * STAGES * Shape::kStage;
+  const uint32_t bars = smem_u32(smem + Shape::kBytes - WARPS * STAGES * 8) + warp * STAGES * 8;
+
+  // the sequence's length and its run of new tokens
+  int len = p.lengths[seq];
+  const int64_t q0 = p.cu != nullptr ? p.cu[seq] : seq;
+  int run = p.cu != nullptr ? p.cu[seq + 1] - p.cu[seq] : 1;
+  const int64_t room = static_cast<int64_t>(p.table.width) * p.table.blocks * kKv4Block;
+  if (len > room) {
+    if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Table);
+    len = static_cast<int>(room);
+  }
+  if (q0 < 0 || run < 0 || q0 + run > p.tokens || run > p.max_tokens) {
+    if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Run);
+    run = q0 < 0 || run < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(min(run, p.max_tokens)), max(p.tokens - q0, int64_t{0})));
+  }
+  const int rows = run * p.group - row_tile * ROWS;   // rows of this tile (may exceed ROWS)
+  if (rows <= 0) return;                              // the same for every CTA of the cluster
+  const int row0 = row_tile * ROWS;
+  // key limit of the tile's last row, in keys; column limits below
+  const int last_tok = min(row0 + ROWS - 1, run * p.group - 1) / p.group;
+  const int first_tok = row0 / p.group;
+  const int seen_most = max(0, min(len, len - run + last_tok + 1));
+  const int seen_least = max(0, min(len, len - run + first_tok + 1));
+  const int tiles = (seen_most + 64 - 1) / 64, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
+
+  if (lane < STAGES) mbar_init(bars + lane * 8, 1);
+  mbar_fence_init();
+  __syncwarp();
+
+  const int first = rank * WARPS + warp, step = splits * WARPS;
+  uint32_t held = 0;      // four bits per stage: which blocks of the tile are there
+  auto issue = [&](int tile, int stage) {
+    const int nb = min(TB, blocks - tile * TB);
+    int64_t at = -1;
+    if (lane < nb) {
+      at = kv4_block_of(p.table, p.kv_heads, seq, tile * TB + lane);
+      if (at < 0) kv4_report(p.status, kDevKv4Table);
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & 15u;
+    if (lane == 0) mbar_expect_tx(bars + stage * 8, __popc(there) * BB);
+    __syncwarp();
+    if (at >= 0)
+      bulk_load(smem_u32(ring + stage * Shape::kStage + lane * BB),
+                p.pages + (at + static_cast<int64_t>(head) * p.table.blocks) * BB, BB, bars + stage * 8);
+    held = (held & ~(15u << (4 * stage))) | (there << (4 * stage));
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (first + s * step < tiles) issue(first + s * step, s);
+
+  // queries as the B operand: column r of n-tile j, scaled to [1, 2) by a power of two; nibbles 1, 3, 5, 7 of a word come
+  // 16 times too large
+  uint32_t qf[NT][G][4];
+  float start[NT][2][G], kcol[NT][2];      // per column 2t, 2t + 1: -8 sum(q) * 2^-24 per group and the factor of S
+  int limit[NT][2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int row = row0 + j * 8 + r, tok = row / p.group;
+    const bool live = tok < run;
+    const T* src = static_cast<const T*>(p.q) + (q0 + tok) * p.q_tok + static_cast<int64_t>(head * p.group + row - tok * p.group) * p.q_head;
+    float x[G][8], big = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (live) kv4_load8(src + 32 * g + 8 * t, p.vec_q, x[g]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!live) x[g][i] = 0.0f;
+        big = fmaxf(big, fabsf(x[g][i]));
+      }
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // exponent of the largest; 100 bounds the factors below (2^(24 + 100) is a finite fp32)
+    const int e = big > 0.0f ? min(100, max(-100, static_cast<int>(__float_as_uint(big) >> 23) - 127)) : 0;
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    float sums[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      sums[g] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[g][i] *= down;
+        sums[g] += x[g][i];
+      }
+      qf[j][g][0] = pack_f16(x[g][0], x[g][4]);
+      qf[j][g][1] = pack_f16(x[g][1] * 0.0625f, x[g][5] * 0.0625f);
+      qf[j][g][2] = pack_f16(x[g][2], x[g][6]);
+      qf[j][g][3] = pack_f16(x[g][3] * 0.0625f, x[g][7] * 0.0625f);
+      sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+      sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+    }
+    const float factor = __uint_as_float(static_cast<uint32_t>(127 + 24 + e) << 23) * p.scale_log2;
+    const int lim = live ? len - run + tok + 1 : 0;
+    // lane (r, t) needs columns 2t and 2t + 1: lanes 4 * (2t) and 4 * (2t + 1) hold them
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int from = 4 * (2 * t + c);
+      kcol[j][c] = __shfl_sync(0xffffffffu, factor, from);
+      limit[j][c] = __shfl_sync(0xffffffffu, lim, from);
+#pragma unroll
+      for (int g = 0; g < G; ++g) start[j][c][g] = __shfl_sync(0xffffffffu, sums[g], from) * (-8.0f / 16777216.0f);
+    }
+  }
+
+  float acc[NT][MT][4], ones[NT][G][4], centre[NT][G][2], top[NT][2], sum[NT][2], norm[G], stepmax[G];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][m][i] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ones[j][g][i] = 0.0f;
+      centre[j][g][0] = centre[j][g][1] = 0.0f;
+    }
+    top[j][0] = top[j][1] = -INFINITY;
+    sum[j][0] = sum[j][1] = 0.0f;
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    norm[g] = 1.0f;
+    stepmax[g] = 0.0f;
+  }
+
+  const int kr = (r >> 1) + 4 * (r & 1);      // row of a block that operand row r stands for; r + 8: kr + 8
+  bool fine = true;
+  uint32_t phase = 0;
+
+  auto consume = [&](auto masked_tag, int tile, int stage) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    const uint8_t* base = ring + stage * Shape::kStage;
+    // scores of the tile: keys kr, kr + 8 of each block, columns 2t, 2t + 1
+    float sc[TB][NT][4];
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      const uint8_t* blk = base + b * BB;
+      uint32_t w0[G], w1[G], m0[G], m1[G];
+      lds_words<G>(w0, blk + kr * (HD / 2) + t * (G * 4));
+      lds_words<G>(w1, blk + (kr + 8) * (HD / 2) + t * (G * 4));
+      lds_words<G>(m0, blk + 8 * HD + kr * (G * 4));
+      lds_words<G>(m1, blk + 8 * HD + (kr + 8) * (G * 4));
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&m0[g]));
+        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&m1[g]));
+        const float ca = a.y * -0.125f, cc = c.y * -0.125f;     // start = -8 sum(q) 2^-24, so c * sum(q) 2^-24 = start * c / -8
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float d[4] = {start[j][0][g], start[j][1][g], start[j][0][g], start[j][1][g]};
+          mma_f16_16816(d, w0[g] & 0x000f000fu, w1[g] & 0x000f000fu, w0[g] & 0x00f000f0u, w1[g] & 0x00f000f0u, qf[j][g][0], qf[j][g][1]);
+          mma_f16_16816(d, (w0[g] >> 8) & 0x000f000fu, (w1[g] >> 8) & 0x000f000fu, (w0[g] >> 8) & 0x00f000f0u,
+                        (w1[g] >> 8) & 0x00f000f0u, qf[j][g][2], qf[j][g][3]);
+          if (g == 0) {
+            sc[b][j][0] = fmaf(ca, start[j][0][g], a.x * d[0]);
+            sc[b][j][1] = fmaf(ca, start[j][1][g], a.x * d[1]);
+            sc[b][j][2] = fmaf(cc, start[j][0][g], c.x * d[2]);
+            sc[b][j][3] = fmaf(cc, start[j][1][g], c.x * d[3]);
+          } else {
+            sc[b][j][0] = fmaf(ca, start[j][0][g], fmaf(a.x, d[0], sc[b][j][0]));
+            sc[b][j][1] = fmaf(ca, start[j][1][g], fmaf(a.x, d[1], sc[b][j][1]));
+            sc[b][j][2] = fmaf(cc, start[j][0][g], fmaf(c.x, d[2], sc[b][j][2]));
+            sc[b][j][3] = fmaf(cc, start[j][1][g], fmaf(c.x, d[3], sc[b][j][3]));
+          }
+        }
+      }
+    }
+    const uint32_t there = (held >> (4 * stage)) & 15u;
+    // running maximum per column
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = sc[b][j][i] * kcol[j][i & 1];
+          if (MASKED) {
+            const int key = tile * 64 + b * 16 + kr + (i >> 1) * 8;
+            if (key >= limit[j][i & 1] || !((there >> b) & 1u)) x = -INFINITY;
+          }
+          sc[b][j][i] = x;
+          most[i & 1] = fmaxf(most[i & 1], x);
+        }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], m));
+        const float now = fmaxf(top[j][c], most[c]);
+        most[c] = now;
+      }
+      if (__any_sync(0xffffffffu, most[0] > top[j][0] || most[1] > top[j][1])) {
+        float alpha[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          alpha[c] = top[j][c] == -INFINITY ? 0.0f : exp2_approx(top[j][c] - most[c]);
+          top[j][c] = most[c];
+          sum[j][c] *= alpha[c];
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][m][i] *= alpha[i & 1];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ones[j][g][i] *= alpha[i & 1];
+          centre[j][g][0] *= alpha[0];
+          centre[j][g][1] *= alpha[1];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float off = top[j][i & 1] == -INFINITY ? 0.0f : top[j][i & 1];
+          sc[b][j][i] = exp2_approx(sc[b][j][i] - off);
+          sum[j][i & 1] += sc[b][j][i];
+        }
+    }
+    // steps of the values: the tile's largest, per group
+    uint32_t v0[TB][G], v1[TB][G];
+    float big[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) big[g] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      const uint8_t* blk = base + b * BB + 18 * HD;
+      lds_words<G>(v0[b], blk + kr * (G * 4));
+      lds_words<G>(v1[b], blk + (kr + 8) * (G * 4));
+      if (MASKED) {
+        const int key = tile * 64 + b * 16 + kr;
+        const bool lost = !((there >> b) & 1u);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if (lost || key >= seen_most) v0[b][g] = 0u;
+          if (lost || key + 8 >= seen_most) v1[b][g] = 0u;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        big[g] = fmaxf(big[g], fmaxf(__low2float(*reinterpret_cast<const __half2*>(&v0[b][g])),
+                                     __low2float(*reinterpret_cast<const __half2*>(&v1[b][g]))));
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (__any_sync(0xffffffffu, big[g] > stepmax[g])) {
+        float now = big[g];
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, m));
+        // the least power of two above it, and its reciprocal
+        const int e = min(120, static_cast<int>(__float_as_uint(now) >> 23) - 126);
+        stepmax[g] = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+        const float next = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        const float beta = next / norm[g];
+        norm[g] = next;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ones[j][g][i] *= beta;
+            acc[j][2 * g][i] *= beta;
+            acc[j][2 * g + 1][i] *= beta;
+          }
+        }
+      }
+    }
+    // output
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      uint32_t pf[NT][G][2];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v0[b][g]));
+        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v1[b][g]));
+        const float sa = a.x * norm[g], sb = c.x * norm[g];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float* x = sc[b][j];
+          float y[4] = {x[0] * sa, x[1] * sa, x[2] * sb, x[3] * sb};
+          float z[4] = {x[0] * a.y, x[1] * a.y, x[2] * c.y, x[3] * c.y};
+          if (MASKED) {      // a hidden key's row may hold anything
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = tile * 64 + b * 16 + kr + (i >> 1) * 8;
+              if (key >= limit[j][i & 1]) y[i] = z[i] = 0.0f;
+            }
+          }
+          centre[j][g][0] += z[0] + z[2];
+          centre[j][g][1] += z[1] + z[3];
+          pf[j][g][0] = transpose_8x8(pack_f16(y[0], y[1]));
+          pf[j][g][1] = transpose_8x8(pack_f16(y[2], y[3]));
+          mma_f16_16816(ones[j][g], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[j][g][0], pf[j][g][1]);
+        }
+      }
+      const uint8_t* blk = base + b * BB + 10 * HD;
+      if constexpr (HD == 32) {
+        const uint16_t* rowp = reinterpret_cast<const uint16_t*>(blk) + r;
+        const uint32_t x = rowp[t * 8] | (static_cast<uint32_t>(rowp[(t + 4) * 8]) << 16);
+        const uint32_t y = rowp[(t + 8) * 8] | (static_cast<uint32_t>(rowp[(t + 12) * 8]) << 16);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_f16_16816(acc[j][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pf[j][0][0], pf[j][0][1]);
+          mma_f16_16816(acc[j][1], (x >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u, (y >> 8) & 0x000f000fu, (y >> 8) & 0x00f000f0u,
+                        pf[j][0][0], pf[j][0][1]);
+        }
+      } else {
+        constexpr int W = HD / 64;
+        uint32_t wa[W], wb[W], wc[W], wd[W];
+        lds_words<W>(wa, blk + t * (HD / 2) + r * (W * 4));
+        lds_words<W>(wb, blk + (t + 4) * (HD / 2) + r * (W * 4));
+        lds_words<W>(wc, blk + (t + 8) * (HD / 2) + r * (W * 4));
+        lds_words<W>(wd, blk + (t + 12) * (HD / 2) + r * (W * 4));
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(wa[w], wb[w], half ? 0x7632 : 0x5410);
+            const uint32_t y = __byte_perm(wc[w], wd[w], half ? 0x7632 : 0x5410);
+            const int m = 4 * w + 2 * half, g = m / 2;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma_f16_16816(acc[j][m], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pf[j][g][0], pf[j][g][1]);
+              mma_f16_16816(acc[j][m + 1], (x >> 8) & 0x000f000fu, (x >> 8) & 0x00f000f0u, (y >> 8) & 0x000f000fu,
+                            (y >> 8) & 0x00f000f0u, pf[j][g][0], pf[j][g][1]);
+            }
+          }
+      }
+    }
+  };
+
+  int stage = 0;
+  for (int tile = first; tile < tiles; tile += step) {
+    if (!mbar_wait(bars + stage * 8, (phase >> stage) & 1u)) { fine = false; break; }
+    phase ^= 1u << stage;
+    if (tile * 64 + 64 > seen_least || ((held >> (4 * stage)) & 15u) != 15u) consume(std::true_type{}, tile, stage);
+    else consume(std::false_type{}, tile, stage);
+    __syncwarp();
+    if (tile + STAGES * step < tiles) issue(tile + STAGES * step, stage);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  if (!fine) {      // give up; the copies still under way end before their shared memory is used for something else
+    if (lane == 0) kv4_report(p.status, kDevKv4Timeout);
+    for (int s = 0; s < STAGES; ++s) mbar_wait(bars + s * 8, (phase >> s) & 1u);
+  }
+
+  // join the warps: each leaves (maximum, sum, output) per row; the ring is free once every warp is here
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem) + warp * (Shape::kPart / 4);
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float s = sum[j][c];
+#pragma unroll
+      for (int m = 4; m < 32; m <<= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+      float ce[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        ce[g] = centre[j][g][c];
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) ce[g] += __shfl_xor_sync(0xffffffffu, ce[g], m);
+      }
+      const int row = j * 8 + 2 * t + c;
+      if (r == 0) {
+        // a NaN sum must survive the join even where no score was a number
+        part[ROWS * HD + row] = s != s ? INFINITY : top[j][c];
+        part[ROWS * HD + ROWS + row] = s;
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int g = m / 2;
+        const float f = 16777216.0f / norm[g];
+        part[row * HD + 16 * m + r] = fmaf(acc[j][m][c] + ones[j][g][c], f, ce[g]);
+        part[row * HD + 16 * m + 8 + r] = fmaf(acc[j][m][c + 2] + ones[j][g][c + 2], f * 0.0625f, ce[g]);
+      }
+    }
+  }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  float* mine = reinterpret_cast<float*>(smem) + WARPS * (Shape::kPart / 4);
+  for (int i = threadIdx.x; i < ROWS * HD; i += WARPS * 32) {
+    const int row = i / HD;
+    float most = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) most = fmaxf(most, all[w * (Shape::kPart / 4) + ROWS * HD + row]);
+    float o = 0.0f, s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float* a = all + w * (Shape::kPart / 4);
+      const float m = a[ROWS * HD + row];
+      if (m == -INFINITY) continue;
+      const float f = exp2_approx(m - most);
+      o = fmaf(f, a[i], o);
+      s = fmaf(f, a[ROWS * HD + ROWS + row], s);
+    }
+    mine[i] = o;
+    if (i % HD == 0) {
+      mine[ROWS * HD + row] = most;
+      mine[ROWS * HD + ROWS + row] = s;
+    }
+  }
+  __syncwarp();
+  if (splits > 1) cluster_sync(); else __syncthreads();
+  const uint32_t mine_at = smem_u32(mine);
+  const int live = min(rows, ROWS);
+  for (int i = rank * WARPS * 32 + threadIdx.x; i < live * HD; i += splits * WARPS * 32) {
+    const int row = i / HD;
+    float o, s;
+    if (splits == 1) {
+      o = mine[i];
+      s = mine[ROWS * HD + ROWS + row];
+    } else {
+      float most = -INFINITY;
+      for (int c = 0; c < splits; ++c) most = fmaxf(most, cluster_ld_f32(mapa_u32(mine_at + (ROWS * HD + row) * 4, c)));
+      o = s = 0.0f;
+      for (int c = 0; c < splits; ++c) {
+        const float m = cluster_ld_f32(mapa_u32(mine_at + (ROWS * HD + row) * 4, c));
+        if (m == -INFINITY) continue;
+        const float f = exp2_approx(m - most);
+        o = fmaf(f, cluster_ld_f32(mapa_u32(mine_at + i * 4, c)), o);
+        s = fmaf(f, cluster_ld_f32(mapa_u32(mine_at + (ROWS * HD + ROWS + row) * 4, c)), s);
+      }
+    }
+    const int at = row0 + row, tok = at / p.group;
+    // a row that sees nothing is zero (its sum is the only one that can be)
+    static_cast<T*>(p.out)[(q0 + tok) * p.o_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.o_head + i % HD] =
+        kv4_from_float<T>(s == 0.0f ? 0.0f : o / s);
+  }
+  __syncwarp();
+  if (splits > 1) cluster_sync();      // nobody leaves while its shared memory is read
+}
+
+}  // namespace crl

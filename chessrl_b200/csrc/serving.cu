@@ -1,0 +1,224 @@
+// Entry points of the decoder-serving operators: the 4-bit key/value cache and next-token logits. See
+// include/chessrl_b200.h for their contracts.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/chessrl_b200.h"
+#include "kv4_append.cuh"
+#include "kv4_attention.cuh"
+#include "logits.cuh"
+
+using namespace crl;
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// rows at multiples of these strides (in 16-bit elements) all start on a 16-byte boundary
+bool rows_aligned(const void* p, int64_t tok, int64_t head) { return aligned16(p) && tok % 8 == 0 && head % 8 == 0; }
+
+int check_cache(const crl_kv4_cache& c) {
+  if (c.pages == nullptr || c.block_table == nullptr || c.num_pages <= 0 || c.kv_heads <= 0 || c.seqs < 0 || c.table_width <= 0 ||
+      c.table_stride < c.table_width)
+    return CRL_ERR_INVALID;
+  if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128) return CRL_ERR_SHAPE;
+  if (c.page_size <= 0 || c.page_size % kKv4Block != 0 || !aligned16(c.pages)) return CRL_ERR_SHAPE;
+  // cache indices are 32-bit, with room for the last tile's end
+  if (static_cast<int64_t>(c.table_width) * c.page_size > INT32_MAX - 1024 || c.num_pages > INT32_MAX) return CRL_ERR_SHAPE;
+  return CRL_OK;
+}
+Kv4Table table_of(const crl_kv4_cache& c) {
+  Kv4Table t;
+  t.table = c.block_table;
+  t.stride = c.table_stride;
+  t.width = c.table_width;
+  t.blocks = c.page_size / kKv4Block;
+  t.num_pages = c.num_pages;
+  return t;
+}
+bool known16(int dtype) { return dtype == CRL_OUT_F16 || dtype == CRL_OUT_BF16; }
+
+template <template <typename, int> class F, typename... A>
+int by_type(int dtype, int hd, A&&... a) {
+  if (dtype == CRL_OUT_F16)
+    return hd == 32 ? F<__half, 32>::run(a...) : hd == 64 ? F<__half, 64>::run(a...) : F<__half, 128>::run(a...);
+  return hd == 32 ? F<__nv_bfloat16, 32>::run(a...) : hd == 64 ? F<__nv_bfloat16, 64>::run(a...) : F<__nv_bfloat16, 128>::run(a...);
+}
+
+int grid_of(int64_t rows, int hd, unsigned* grid) {
+  const int64_t blocks = (rows * (hd / 8) + 255) / 256;
+  if (blocks > INT32_MAX) return CRL_ERR_SHAPE;
+  *grid = static_cast<unsigned>(blocks);
+  return CRL_OK;
+}
+
+template <typename T, int HD>
+struct Append {
+  static int run(const Kv4AppendParams& p, cudaStream_t s) {
+    unsigned grid;
+    if (grid_of(p.tokens * (p.heads + 2 * p.kv_heads), HD, &grid) != CRL_OK) return CRL_ERR_SHAPE;
+    kv4_append_kernel<T, HD><<<grid, 256, 0, s>>>(p);
+    return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
+  }
+};
+template <typename T, int HD>
+struct Read {
+  static int run(const Kv4ReadParams& p, cudaStream_t s) {
+    unsigned grid;
+    if (grid_of(p.tokens * 2 * p.kv_heads, HD, &grid) != CRL_OK) return CRL_ERR_SHAPE;
+    kv4_read_kernel<T, HD><<<grid, 256, 0, s>>>(p);
+    return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
+  }
+};
+
+template <typename T, int HD, int NT>
+int attend_rows(Kv4AttentionParams p, int sms, int64_t max_keys, cudaStream_t s) {
+  constexpr int WARPS = 8, STAGES = HD == 32 ? 3 : 2;
+  using Shape = Kv4AttnShape<HD, NT, WARPS, STAGES>;
+  auto* kernel = kv4_attention_kernel<T, HD, NT, WARPS, STAGES>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes) != cudaSuccess) return CRL_ERR_CUDA;
+  p.row_tiles = (p.max_tokens * p.group + Shape::kRows - 1) / Shape::kRows;
+  const int64_t units = static_cast<int64_t>(p.seqs) * p.kv_heads * p.row_tiles;
+  // the axis of keys is split over a cluster while there are SMs without work and tiles for every warp
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= 2 * sms && static_cast<int64_t>(splits) * 2 * WARPS * 64 <= max_keys) splits *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(splits, p.kv_heads * p.row_tiles, p.seqs);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = Shape::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<const Kv4AttentionParams>(p)) == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
+}
+template <typename T, int HD>
+struct Attend {
+  static int run(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
+    if (static_cast<int64_t>(p.max_tokens) * p.group <= 8) return attend_rows<T, HD, 1>(p, sms, max_keys, s);
+    return attend_rows<T, HD, 2>(p, sms, max_keys, s);
+  }
+};
+
+template <typename T>
+int logits_rows(const LogitsParams& p, cudaStream_t s) {
+  const int64_t grid = p.rows * p.tiles;
+  if (grid > INT32_MAX) return CRL_ERR_SHAPE;
+  adjust_logits_kernel<T><<<static_cast<unsigned>(grid), kLogitsThreads, p.tile * 4, s>>>(p);
+  return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t crl_kv4_page_bytes(int32_t page_size, int32_t kv_heads, int32_t head_dim) {
+  if (page_size <= 0 || page_size % kKv4Block != 0 || kv_heads <= 0 || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
+  return static_cast<size_t>(kv_heads) * (page_size / kKv4Block) * kv4_block_bytes(head_dim);
+}
+
+int crl_kv4_append(const crl_kv4_append_args* a) {
+  if (a == nullptr) return CRL_ERR_INVALID;
+  if (const int rc = check_cache(a->cache)) return rc;
+  const crl_kv4_cache& c = a->cache;
+  if (a->k == nullptr || a->v == nullptr || a->starts == nullptr || a->tokens < 0 || a->heads < 0 || !known16(a->dtype)) return CRL_ERR_INVALID;
+  if (a->heads > 0 && (a->q == nullptr || a->q_out == nullptr || a->q == a->q_out)) return CRL_ERR_INVALID;
+  if (a->rope != nullptr && (a->rope_dim <= 0 || a->rope_dim % 2 != 0 || a->rope_dim > c.head_dim || a->rope_positions <= 0))
+    return CRL_ERR_SHAPE;
+  if (a->tokens == 0 || c.seqs == 0) return CRL_OK;
+  Kv4AppendParams p{};
+  p.pages = static_cast<uint8_t*>(c.pages);
+  p.table = table_of(c);
+  p.starts = a->starts; p.cu = a->cu_tokens; p.seqs = c.seqs; p.kv_heads = c.kv_heads; p.heads = a->heads; p.tokens = a->tokens;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out;
+  p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.k_tok = a->k_token_stride; p.k_head = a->k_head_stride;
+  p.v_tok = a->v_token_stride; p.v_head = a->v_head_stride; p.o_tok = a->out_token_stride; p.o_head = a->out_head_stride;
+  p.rope = reinterpret_cast<const float2*>(a->rope); p.rope_positions = a->rope_positions; p.rot = a->rope_dim;
+  p.interleaved = a->rope_interleaved;
+  p.vec_q = rows_aligned(a->q, p.q_tok, p.q_head); p.vec_k = rows_aligned(a->k, p.k_tok, p.k_head);
+  p.vec_v = rows_aligned(a->v, p.v_tok, p.v_head); p.vec_o = rows_aligned(a->q_out, p.o_tok, p.o_head);
+  p.status = a->device_status;
+  return by_type<Append>(a->dtype, c.head_dim, p, static_cast<cudaStream_t>(a->stream));
+}
+
+int crl_kv4_read(const crl_kv4_read_args* a) {
+  if (a == nullptr) return CRL_ERR_INVALID;
+  if (const int rc = check_cache(a->cache)) return rc;
+  const crl_kv4_cache& c = a->cache;
+  if (a->k == nullptr || a->v == nullptr || a->starts == nullptr || a->tokens < 0 || !known16(a->dtype)) return CRL_ERR_INVALID;
+  if (a->tokens == 0 || c.seqs == 0) return CRL_OK;
+  Kv4ReadParams p{};
+  p.pages = static_cast<const uint8_t*>(c.pages);
+  p.table = table_of(c);
+  p.starts = a->starts; p.cu = a->cu_tokens; p.seqs = c.seqs; p.kv_heads = c.kv_heads; p.tokens = a->tokens;
+  p.k = a->k; p.v = a->v;
+  p.k_tok = a->k_token_stride; p.k_head = a->k_head_stride; p.v_tok = a->v_token_stride; p.v_head = a->v_head_stride;
+  p.vec_k = rows_aligned(a->k, p.k_tok, p.k_head); p.vec_v = rows_aligned(a->v, p.v_tok, p.v_head);
+  p.status = a->device_status;
+  return by_type<Read>(a->dtype, c.head_dim, p, static_cast<cudaStream_t>(a->stream));
+}
+
+int crl_kv4_attention(const crl_kv4_attention_args* a) {
+  if (a == nullptr) return CRL_ERR_INVALID;
+  if (const int rc = check_cache(a->cache)) return rc;
+  const crl_kv4_cache& c = a->cache;
+  if (a->q == nullptr || a->out == nullptr || a->lengths == nullptr || a->tokens < 0 || !known16(a->dtype) || a->heads <= 0 ||
+      a->max_tokens < 0)
+    return CRL_ERR_INVALID;
+  if (a->heads % c.kv_heads != 0 || c.seqs > 65535) return CRL_ERR_SHAPE;
+  if (a->tokens == 0 || c.seqs == 0 || a->max_tokens == 0) return CRL_OK;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return CRL_ERR_CUDA;
+  Kv4AttentionParams p{};
+  p.pages = static_cast<const uint8_t*>(c.pages);
+  p.table = table_of(c);
+  p.lengths = a->lengths; p.cu = a->cu_tokens; p.seqs = c.seqs; p.kv_heads = c.kv_heads; p.group = a->heads / c.kv_heads;
+  p.max_tokens = a->cu_tokens != nullptr ? static_cast<int32_t>(std::min<int64_t>(a->max_tokens, a->tokens)) : 1;
+  if (static_cast<int64_t>(p.max_tokens) * p.group / 8 * c.kv_heads > 65535 - c.kv_heads) return CRL_ERR_SHAPE;
+  p.tokens = a->tokens;
+  p.q = a->q; p.out = a->out;
+  p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.o_tok = a->out_token_stride; p.o_head = a->out_head_stride;
+  p.vec_q = rows_aligned(a->q, p.q_tok, p.q_head);
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.status = a->device_status;
+  return by_type<Attend>(a->dtype, c.head_dim, p, sms, static_cast<int64_t>(c.table_width) * c.page_size,
+                         static_cast<cudaStream_t>(a->stream));
+}
+
+int crl_adjust_logits(const crl_logits_args* a) {
+  if (a == nullptr || a->in == nullptr || a->out == nullptr) return CRL_ERR_INVALID;
+  if (a->dtype != CRL_OUT_F32 && !known16(a->dtype)) return CRL_ERR_INVALID;
+  if (a->rows < 0 || a->vocab <= 0 || a->in_stride < a->vocab || a->out_stride < a->vocab || a->history_len < 0 || a->biases < 0)
+    return CRL_ERR_INVALID;
+  if ((a->history_len > 0 && (a->history == nullptr || a->history_stride < a->history_len)) ||
+      (a->biases > 0 && (a->bias_ids == nullptr || a->bias_values == nullptr || a->bias_stride < a->biases || a->value_stride < a->biases)))
+    return CRL_ERR_INVALID;
+  if (a->history_len > kLogitsMaxHistory || a->biases > kLogitsMaxBiases || a->vocab > INT32_MAX - 65536) return CRL_ERR_SHAPE;
+  if (a->mask != nullptr && (a->mask_count <= 0 || a->mask_stride < (static_cast<int64_t>(a->vocab) + 7) / 8)) return CRL_ERR_INVALID;
+  if (a->mask != nullptr && a->mask_rows == nullptr && a->mask_count < a->rows) return CRL_ERR_INVALID;
+  if (a->rows == 0) return CRL_OK;
+  const int size = a->dtype == CRL_OUT_F32 ? 4 : 2;
+  LogitsParams p{};
+  p.in = a->in; p.out = a->out; p.in_stride = a->in_stride; p.out_stride = a->out_stride; p.rows = a->rows; p.vocab = a->vocab;
+  p.history = a->history_len > 0 ? a->history : nullptr; p.history_stride = a->history_stride; p.history_len = a->history_len;
+  p.repetition = a->repetition; p.frequency = a->frequency; p.presence = a->presence;
+  p.bias_ids = a->bias_ids; p.bias_values = a->bias_values; p.bias_stride = a->bias_stride; p.value_stride = a->value_stride;
+  p.biases = a->biases;
+  p.mask = a->mask; p.mask_stride = a->mask_stride; p.mask_count = static_cast<int32_t>(std::min<int64_t>(a->mask_count, INT32_MAX));
+  p.mask_rows = a->mask_rows; p.masked_value = a->masked_value; p.status = a->device_status;
+  const intptr_t ip = reinterpret_cast<intptr_t>(a->in), op = reinterpret_cast<intptr_t>(a->out);
+  p.same_phase = (ip - op) % 16 == 0 && ((a->in_stride - a->out_stride) * size) % 16 == 0 && ip % size == 0;
+  p.tile = 4096;
+  p.tiles = (p.vocab + p.tile - 1) / p.tile;
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  if (a->dtype == CRL_OUT_F32) return logits_rows<float>(p, s);
+  if (a->dtype == CRL_OUT_F16) return logits_rows<__half>(p, s);
+  return logits_rows<__nv_bfloat16>(p, s);
+}
+
+}  // extern "C"

@@ -55,7 +55,7 @@ enum { CRL_MASK_NONE = 0, CRL_MASK_BITS = 1, CRL_MASK_ADDITIVE = 2, CRL_MASK_FRO
 /* CRL_MASK_FROM_RECORDS (input layout CRL_LAYOUT_PACKED104, 1858-move gather head): the library generates the
  * legal moves of every position on the device from its packed record and masks like CRL_MASK_BITS; legal_mask
  * is ignored. Stands for the python-chess loop of model_bis.py:373-380 / pgn_to_input_data_decoder.py:35-42. */
-enum { CRL_OUT_F32 = 0, CRL_OUT_F16 = 1 };
+enum { CRL_OUT_F32 = 0, CRL_OUT_F16 = 1, CRL_OUT_BF16 = 2 };   /* BF16: decoder-serving operators only */
 enum { CRL_VOCAB_NATIVE = 0, CRL_VOCAB_RL1929 = 1 };
 
 /* Network description. Stands for the reference constructors
@@ -272,6 +272,126 @@ typedef struct crl_linear_args {
                               row maximum / 127 as the scale, written here, [m] f32); required with lno_x8 then */
 } crl_linear_args;
 int crl_linear_ex(const crl_linear_args* args);
+
+/* ---- decoder serving: a 4-bit key/value cache and next-token logits ------------------------------------------------
+ * What a decoder like model_bis.py's GPT needs to continue a sequence without recomputing its prefix (its
+ * generate_sequence_raw, model_bis.py:272-320, has no cache). Operators without a handle, like crl_linear_ex: device
+ * pointers of the current device, work enqueued on `stream`, no workspace, no allocation, no synchronisation, so a call
+ * can be captured into a CUDA graph and calls on different streams do not disturb one another. `device_status`
+ * (nullable, one int of device memory, zero before the call) receives a code when a kernel had to skip something:
+ *   121 a cache index outside the sequence's row of the block table, or a page number outside the pool;
+ *   122 a sequence with more new tokens than max_tokens, or token rows past the tensor;
+ *   123 a position past the rotation table;   124 a bounded wait ran out;
+ *   131 a row asks for a mask that the table does not have.
+ * Nothing is read or written out of bounds in any of these cases.
+ *
+ * The cache is a pool of pages; a sequence's cache index i lies in page block_table[seq, i / page_size]. A (token, head)
+ * row is held in groups of 32 values: a step s and a centre c in f16 and a 4-bit code n per value, which stands for
+ * (n - 8) * s + c. With lo / hi the group's extremes: s = f16(bf16((hi - lo) * (1 / 15))), c = f16(lo + 8 s),
+ * n = clamp(rint((x - c) * (1 / s)) + 8, 0, 15) in fp32 (1 / 15 and 1 / s rounded to fp32 first), n = 8 where s = 0. Values beyond +-57344 are held as that; a NaN
+ * makes its group NaN. A page is [kv_heads][page_size / 16] blocks of 16 tokens, a block = 20 * head_dim bytes:
+ *   key codes [16][hd/2] | key (s, c) [16][hd/32] | value codes [16][hd/2] | value (s, c) [16][hd/32]; nibble p of a row
+ *   (low half of a byte first) is dim 32 g + 8 t + i of a key, p = (t, g, i) with t < 4, g < hd/32, i < 8, and dim
+ *   8 i + r of a value, p = (r, i) with r < 8, i < hd/8.
+ * head_dim 32, 64 or 128; page_size a multiple of 16; pages 16-byte aligned. A page may appear in the tables of several
+ * sequences (a shared prefix) as long as no call appends to it twice. */
+typedef struct crl_kv4_cache {
+  void* pages;                 /* [num_pages] x crl_kv4_page_bytes */
+  int64_t num_pages;
+  int32_t page_size;           /* tokens */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t seqs;
+  const int32_t* block_table;  /* [seqs, table_stride] page numbers; only those of indices in use are looked at */
+  int64_t table_stride;
+  int32_t table_width;         /* pages a sequence may have */
+} crl_kv4_cache;
+/* Bytes of a page, 0 for a shape that is not supported. */
+size_t crl_kv4_page_bytes(int32_t page_size, int32_t kv_heads, int32_t head_dim);
+
+/* Appends the new tokens' keys and values (rotated on the way when `rope` is given) and rotates their queries. Token
+ * rows cu_tokens[s] .. cu_tokens[s + 1] - 1 belong to sequence s and take cache indices starts[s], starts[s] + 1, ...;
+ * without cu_tokens row s is the one new token of sequence s. Rows behind the last sequence are left alone.
+ * Rotation of the first rope_dim dims at position p (= cache index), table entry (cos, sin) per pair:
+ *   halves: pair i = dims i, i + rope_dim / 2; interleaved: dims 2i, 2i + 1;  (a, b) -> (a cos - b sin, b cos + a sin),
+ * evaluated in twice fp32's precision and rounded once. Strides are in elements; the dims of a row are contiguous. */
+typedef struct crl_kv4_append_args {
+  crl_kv4_cache cache;
+  int32_t dtype;               /* CRL_OUT_F16 / CRL_OUT_BF16 of q, k, v and q_out */
+  int32_t heads;               /* rows of q per token; 0: no queries */
+  int64_t tokens;              /* token rows of q, k, v */
+  const void* q; int64_t q_token_stride; int64_t q_head_stride;
+  const void* k; int64_t k_token_stride; int64_t k_head_stride;
+  const void* v; int64_t v_token_stride; int64_t v_head_stride;
+  void* q_out; int64_t out_token_stride; int64_t out_head_stride;   /* must not overlap q */
+  const int32_t* starts;       /* [seqs] */
+  const int32_t* cu_tokens;    /* nullable, [seqs + 1] ascending from 0 */
+  const float* rope;           /* nullable, [rope_positions, rope_dim / 2, 2] */
+  int64_t rope_positions;
+  int32_t rope_dim;            /* even, <= head_dim */
+  int32_t rope_interleaved;
+  int* device_status;
+  void* stream;
+} crl_kv4_append_args;
+int crl_kv4_append(const crl_kv4_append_args* args);
+
+/* The values that the cache holds for the same rows (cache indices starts[s] + j), rounded to `dtype`. */
+typedef struct crl_kv4_read_args {
+  crl_kv4_cache cache;
+  int32_t dtype;
+  int64_t tokens;
+  void* k; int64_t k_token_stride; int64_t k_head_stride;
+  void* v; int64_t v_token_stride; int64_t v_head_stride;
+  const int32_t* starts;
+  const int32_t* cu_tokens;
+  int* device_status;
+  void* stream;
+} crl_kv4_read_args;
+int crl_kv4_read(const crl_kv4_read_args* args);
+
+/* out = softmax(scale * q K^T) V over the cache, causal (model_bis.py:71 with the prefix's keys and values taken from the
+ * cache): a sequence's new tokens are its last ones, new token j of n at length L sees cache indices 0 .. L - n + j. A row
+ * that sees nothing is zero. heads is a multiple of kv_heads; query head h reads key head h / (heads / kv_heads). */
+typedef struct crl_kv4_attention_args {
+  crl_kv4_cache cache;
+  int32_t dtype;               /* CRL_OUT_F16 / CRL_OUT_BF16 of q and out */
+  int32_t heads;
+  int64_t tokens;              /* token rows of q and out */
+  const void* q; int64_t q_token_stride; int64_t q_head_stride;
+  void* out; int64_t out_token_stride; int64_t out_head_stride;
+  const int32_t* lengths;      /* [seqs] cached tokens, the new ones included */
+  const int32_t* cu_tokens;    /* nullable: one new token per sequence */
+  int32_t max_tokens;          /* most new tokens of any sequence (sizes the launch) */
+  float scale;
+  int* device_status;
+  void* stream;
+} crl_kv4_attention_args;
+int crl_kv4_attention(const crl_kv4_attention_args* args);
+
+/* Next-token logits before a move is drawn from them: with z = in[row, v] and n = how often v stands in the row's history
+ *   n > 0: z = (z > 0 ? z / repetition : z * repetition) - (frequency * n + presence);   z += bias of v;
+ *   bit v of the row's mask clear: z = masked_value.
+ * fp32, each operation rounded once. The bitsets are those of crl_legal_mask_1929 / crl_legal_masks_packed104. Entries of
+ * history and bias_ids outside the vocabulary are padding; of equal bias ids in a row the last one counts. out may be in. */
+typedef struct crl_logits_args {
+  int32_t dtype;               /* CRL_OUT_F32 / CRL_OUT_F16 / CRL_OUT_BF16 of in and out */
+  int32_t vocab;
+  int64_t rows;
+  const void* in; int64_t in_stride;
+  void* out; int64_t out_stride;
+  const int32_t* history; int64_t history_stride; int32_t history_len;   /* [rows, history_len], up to 2^20 - 1 */
+  const float* repetition;     /* nullable, [rows]; default 1 */
+  const float* frequency;      /* nullable, [rows]; default 0 */
+  const float* presence;       /* nullable, [rows]; default 0 */
+  const int32_t* bias_ids; int64_t bias_stride;                          /* [rows, biases], up to 4094 */
+  const float* bias_values; int64_t value_stride; int32_t biases;
+  const uint8_t* mask; int64_t mask_stride; int64_t mask_count;          /* [mask_count, mask_stride] bitsets */
+  const int32_t* mask_rows;    /* nullable, [rows]: which bitset a row takes, negative: none; null: row r takes bitset r */
+  float masked_value;
+  int* device_status;
+  void* stream;
+} crl_logits_args;
+int crl_adjust_logits(const crl_logits_args* args);
 
 /* ---- host-side input producers (no GPU needed) ------------------------------------------------------------
  * The reference builds its inputs with python-chess; these entry points are the library's own rules
