@@ -116,7 +116,7 @@ class Kv4AttentionArgs(ctypes.Structure):
 
 class LogitsArgs(ctypes.Structure):
     """Mirror of `crl_logits_args`."""
-    _fields_ = [("dtype", _I32), ("vocab", _I32), ("rows", _I64), ("in", _P), ("in_stride", _I64),
+    _fields_ = [("dtype", _I32), ("vocab", _I32), ("rows", _I64), ("logits", _P), ("in_stride", _I64),
                 ("out", _P), ("out_stride", _I64), ("history", _P), ("history_stride", _I64), ("history_len", _I32),
                 ("repetition", _P), ("frequency", _P), ("presence", _P),
                 ("bias_ids", _P), ("bias_stride", _I64), ("bias_values", _P), ("value_stride", _I64), ("biases", _I32),

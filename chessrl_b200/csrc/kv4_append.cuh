@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
   const int lane = threadIdx.x & 31, part = lane % LANES;
   const int per_token = 2 * p.kv_heads;
   const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
-  bool ok = unit < p.tokens * per_token;
+  const bool live = unit < p.tokens * per_token;
+  bool ok = live;
   const int64_t tok = ok ? unit / per_token : 0;
   int h = ok ? static_cast<int>(unit - tok * per_token) : 0;
   int seq = 0;
@@ -232,9 +233,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     const int pos = r * LANES + part;        // values: nibble position of dim 8 * part + r
     const uint32_t w = __shfl_sync(0xffffffffu, word, (lane - part) + pos / 8);
     const uint32_t n = is_k ? word >> (4 * r) : w >> (4 * (pos % 8));
-    x[r] = __fmaf_rn(static_cast<float>(static_cast<int>(n & 15u) - 8), s, c);
+    x[r] = __fmaf_rn(static_cast<float>(static_cast<int>(n & 15u) - 8), s, c);      // no row: s = c = 0
   }
-  if (!ok) return;
+  if (!live) return;
   T* out = is_k ? static_cast<T*>(p.k) + tok * p.k_tok + static_cast<int64_t>(h) * p.k_head
                 : static_cast<T*>(p.v) + tok * p.v_tok + static_cast<int64_t>(h) * p.v_head;
   kv4_store8(out + part * 8, is_k ? p.vec_k : p.vec_v, x);

@@ -3,10 +3,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/chessrl_b200.h"
 #include "kv4_append.cuh"
 #include "kv4_attention.cuh"
+#include "kv4_rows.cuh"
 #include "logits.cuh"
 
 using namespace crl;
@@ -46,6 +48,20 @@ int by_type(int dtype, int hd, A&&... a) {
   return hd == 32 ? F<__nv_bfloat16, 32>::run(a...) : hd == 64 ? F<__nv_bfloat16, 64>::run(a...) : F<__nv_bfloat16, 128>::run(a...);
 }
 
+// SMs of the current device, asked once per device
+int current_sms(int* sms) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return CRL_ERR_CUDA;
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return CRL_ERR_CUDA;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  }
+  *sms = n;
+  return CRL_OK;
+}
+
 int grid_of(int64_t rows, int hd, unsigned* grid) {
   const int64_t blocks = (rows * (hd / 8) + 255) / 256;
   if (blocks > INT32_MAX) return CRL_ERR_SHAPE;
@@ -72,21 +88,27 @@ struct Read {
   }
 };
 
-template <typename T, int HD, int NT>
-int attend_rows(Kv4AttentionParams p, int sms, int64_t max_keys, cudaStream_t s) {
-  constexpr int WARPS = 8, STAGES = HD == 32 ? 3 : 2;
-  using Shape = Kv4AttnShape<HD, NT, WARPS, STAGES>;
-  auto* kernel = kv4_attention_kernel<T, HD, NT, WARPS, STAGES>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes) != cudaSuccess) return CRL_ERR_CUDA;
-  p.row_tiles = (p.max_tokens * p.group + Shape::kRows - 1) / Shape::kRows;
+// One launch of an attention kernel: a cluster of `splits` CTAs along the keys per (row tile, key head, sequence).
+template <typename K>
+int attend_launch(K* kernel, std::atomic<uint64_t>& ready, int bytes, int threads, int tile_rows, int keys_at_once, int resident,
+                  Kv4AttentionParams p, int sms, int64_t max_keys, cudaStream_t s) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return CRL_ERR_CUDA;
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {      // once per kernel and device
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return CRL_ERR_CUDA;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  p.row_tiles = (p.max_tokens * p.group + tile_rows - 1) / tile_rows;
   const int64_t units = static_cast<int64_t>(p.seqs) * p.kv_heads * p.row_tiles;
+  if (static_cast<int64_t>(p.kv_heads) * p.row_tiles > 65535) return CRL_ERR_SHAPE;
   // the axis of keys is split over a cluster while there are SMs without work and tiles for every warp
   int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 2 * sms && static_cast<int64_t>(splits) * 2 * WARPS * 64 <= max_keys) splits *= 2;
+  while (splits < 8 && units * splits * 2 <= resident * sms && static_cast<int64_t>(splits) * 2 * keys_at_once <= max_keys) splits *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, p.kv_heads * p.row_tiles, p.seqs);
-  cfg.blockDim = dim3(WARPS * 32);
-  cfg.dynamicSmemBytes = Shape::kBytes;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -97,10 +119,27 @@ int attend_rows(Kv4AttentionParams p, int sms, int64_t max_keys, cudaStream_t s)
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const Kv4AttentionParams>(p)) == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
 }
 template <typename T, int HD>
+int attend_few(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
+  constexpr int WARPS = 8, STAGES = HD == 32 ? 3 : 2;
+  using Shape = Kv4AttnShape<HD, 1, WARPS, STAGES>;
+  static std::atomic<uint64_t> ready{0};
+  return attend_launch(kv4_attention_kernel<T, HD, 1, WARPS, STAGES>, ready, Shape::kBytes, WARPS * 32, Shape::kRows, WARPS * 64, 2, p,
+                       sms, max_keys, s);
+}
+template <typename T, int HD, int RW>
+int attend_rows(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
+  using Shape = Kv4RowsShape<HD, RW, 4 / RW>;
+  static std::atomic<uint64_t> ready{0};
+  return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, ready, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, 2, p, sms, max_keys, s);
+}
+template <typename T, int HD>
 struct Attend {
   static int run(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
-    if (static_cast<int64_t>(p.max_tokens) * p.group <= 8) return attend_rows<T, HD, 1>(p, sms, max_keys, s);
-    return attend_rows<T, HD, 2>(p, sms, max_keys, s);
+    const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group;
+    if (rows <= 8) return attend_few<T, HD>(p, sms, max_keys, s);
+    if (rows <= 16) return attend_rows<T, HD, 1>(p, sms, max_keys, s);
+    if (rows <= 32) return attend_rows<T, HD, 2>(p, sms, max_keys, s);
+    return attend_rows<T, HD, 4>(p, sms, max_keys, s);
   }
 };
 
@@ -171,19 +210,19 @@ int crl_kv4_attention(const crl_kv4_attention_args* a) {
     return CRL_ERR_INVALID;
   if (a->heads % c.kv_heads != 0 || c.seqs > 65535) return CRL_ERR_SHAPE;
   if (a->tokens == 0 || c.seqs == 0 || a->max_tokens == 0) return CRL_OK;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return CRL_ERR_CUDA;
+  int sms = 0;
+  if (const int rc = current_sms(&sms)) return rc;
   Kv4AttentionParams p{};
   p.pages = static_cast<const uint8_t*>(c.pages);
   p.table = table_of(c);
   p.lengths = a->lengths; p.cu = a->cu_tokens; p.seqs = c.seqs; p.kv_heads = c.kv_heads; p.group = a->heads / c.kv_heads;
   p.max_tokens = a->cu_tokens != nullptr ? static_cast<int32_t>(std::min<int64_t>(a->max_tokens, a->tokens)) : 1;
-  if (static_cast<int64_t>(p.max_tokens) * p.group / 8 * c.kv_heads > 65535 - c.kv_heads) return CRL_ERR_SHAPE;
+  if (static_cast<int64_t>(p.max_tokens) * p.group > INT32_MAX - 256) return CRL_ERR_SHAPE;
   p.tokens = a->tokens;
   p.q = a->q; p.out = a->out;
   p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.o_tok = a->out_token_stride; p.o_head = a->out_head_stride;
   p.vec_q = rows_aligned(a->q, p.q_tok, p.q_head);
+  p.pair_o = (reinterpret_cast<uintptr_t>(a->out) & 3) == 0 && p.o_tok % 2 == 0 && p.o_head % 2 == 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.status = a->device_status;
   return by_type<Attend>(a->dtype, c.head_dim, p, sms, static_cast<int64_t>(c.table_width) * c.page_size,
@@ -191,7 +230,7 @@ int crl_kv4_attention(const crl_kv4_attention_args* a) {
 }
 
 int crl_adjust_logits(const crl_logits_args* a) {
-  if (a == nullptr || a->in == nullptr || a->out == nullptr) return CRL_ERR_INVALID;
+  if (a == nullptr || a->logits == nullptr || a->out == nullptr) return CRL_ERR_INVALID;
   if (a->dtype != CRL_OUT_F32 && !known16(a->dtype)) return CRL_ERR_INVALID;
   if (a->rows < 0 || a->vocab <= 0 || a->in_stride < a->vocab || a->out_stride < a->vocab || a->history_len < 0 || a->biases < 0)
     return CRL_ERR_INVALID;
@@ -204,14 +243,14 @@ int crl_adjust_logits(const crl_logits_args* a) {
   if (a->rows == 0) return CRL_OK;
   const int size = a->dtype == CRL_OUT_F32 ? 4 : 2;
   LogitsParams p{};
-  p.in = a->in; p.out = a->out; p.in_stride = a->in_stride; p.out_stride = a->out_stride; p.rows = a->rows; p.vocab = a->vocab;
+  p.in = a->logits; p.out = a->out; p.in_stride = a->in_stride; p.out_stride = a->out_stride; p.rows = a->rows; p.vocab = a->vocab;
   p.history = a->history_len > 0 ? a->history : nullptr; p.history_stride = a->history_stride; p.history_len = a->history_len;
   p.repetition = a->repetition; p.frequency = a->frequency; p.presence = a->presence;
   p.bias_ids = a->bias_ids; p.bias_values = a->bias_values; p.bias_stride = a->bias_stride; p.value_stride = a->value_stride;
   p.biases = a->biases;
   p.mask = a->mask; p.mask_stride = a->mask_stride; p.mask_count = static_cast<int32_t>(std::min<int64_t>(a->mask_count, INT32_MAX));
   p.mask_rows = a->mask_rows; p.masked_value = a->masked_value; p.status = a->device_status;
-  const intptr_t ip = reinterpret_cast<intptr_t>(a->in), op = reinterpret_cast<intptr_t>(a->out);
+  const intptr_t ip = reinterpret_cast<intptr_t>(a->logits), op = reinterpret_cast<intptr_t>(a->out);
   p.same_phase = (ip - op) % 16 == 0 && ((a->in_stride - a->out_stride) * size) % 16 == 0 && ip % size == 0;
   p.tile = 4096;
   p.tiles = (p.vocab + p.tile - 1) / p.tile;

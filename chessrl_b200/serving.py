@@ -21,87 +21,101 @@ import torch
 
 from . import _lib as L
 
+_Tensor = torch.Tensor
 _DTYPE = {torch.float32: L.OUT_F32, torch.float16: L.OUT_F16, torch.bfloat16: L.OUT_BF16}
 _HALF = (torch.float16, torch.bfloat16)
+_ANY, _I32, _U8, _F32 = tuple(_DTYPE), (torch.int32,), (torch.uint8,), (torch.float32,)
+
+# A call for one token takes the GPU a few microseconds, so the host side counts: checks are single expressions whose
+# message is only put together where one fails, and the stream is taken by its number.
 
 
-def _call(name, args, device):
+def _call(name, args, index):
     lib = L.load()
-    if torch.cuda.current_device() == device.index:
-        args.stream = torch.cuda.current_stream(device).cuda_stream
+    args.stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
         rc = getattr(lib, name)(ctypes.byref(args))
     else:
-        with torch.cuda.device(device):
-            args.stream = torch.cuda.current_stream(device).cuda_stream
+        with torch.cuda.device(index):
             rc = getattr(lib, name)(ctypes.byref(args))
     if rc != 0:
         raise L.CrlError(rc, name)
 
 
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
-
-
-def _check(name, t, device, dtypes, dim):
-    """`t` is a tensor of `dim` dimensions on `device` with one of `dtypes`: the library gets raw pointers and sees none
+def _check(name, t, index, dtypes, dim):
+    """`t` is a tensor of `dim` dimensions on GPU `index` with one of `dtypes`: the library gets raw pointers and sees none
     of this."""
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(t.device == device, f"{name} must live on {device}, got {t.device}")
-    _need(t.dtype in dtypes, f"{name} must have dtype {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    _need(t.dim() == dim, f"{name} must have {dim} dimensions, got shape {tuple(t.shape)}")
+    if isinstance(t, _Tensor) and t.get_device() == index and t.dtype in dtypes and t.dim() == dim:
+        return
+    if not isinstance(t, _Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must live on cuda:{index}, got {t.device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must have dtype {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    raise ValueError(f"{name} must have {dim} dimensions, got shape {tuple(t.shape)}")
 
 
-def _ints(name, t, device, count):
-    _check(name, t, device, (torch.int32,), 1)
-    _need(t.shape[0] == count and (count <= 1 or t.stride(0) == 1), f"{name} must hold {count} contiguous int32, got shape {tuple(t.shape)}")
+def _vector(name, t, index, count, dtypes=_I32):
+    _check(name, t, index, dtypes, 1)
+    if t.shape[0] != count or count > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} must hold {count} contiguous {str(dtypes[0])[6:]}, got shape {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _status(status, device):
+def _status(status, index):
     if status is None:
         return None
-    _check("status", status, device, (torch.int32,), 1)
-    _need(status.shape[0] >= 1, "status must hold an int32")
+    _check("status", status, index, _I32, 1)
+    if status.shape[0] < 1:
+        raise ValueError("status must hold an int32")
     return status.data_ptr()
 
 
-def _rows(name, t, device, dtypes, heads, dim):
-    _check(name, t, device, dtypes, 3)
-    _need(t.shape[2] == dim and (heads is None or t.shape[1] == heads),
-          f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}], got shape {tuple(t.shape)}")
-    _need(t.stride(2) == 1, f"the last dimension of {name} must be contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+def _rows(name, t, index, dtypes, heads, dim):
+    _check(name, t, index, dtypes, 3)
+    shape, stride = t.shape, t.stride()
+    if shape[2] != dim or heads is not None and shape[1] != heads:
+        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}], got shape {tuple(shape)}")
+    if stride[2] != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    return t.data_ptr(), stride[0], stride[1]
 
 
 def kv4_pages(num_pages, page_size, kv_heads, head_dim, device="cuda"):
     """A pool of cache pages: uint8 [num_pages, kv_heads, page_size / 16, 20 * head_dim]. Its shape says everything about
     the cache; page_size is a multiple of 16, head_dim 32, 64 or 128."""
-    _need(L.load().crl_kv4_page_bytes(page_size, kv_heads, head_dim) > 0,
-          f"no 4-bit pages of {page_size} tokens, {kv_heads} heads of {head_dim}: page_size is a multiple of 16, head_dim 32, 64 or 128")
+    if L.load().crl_kv4_page_bytes(page_size, kv_heads, head_dim) == 0:
+        raise ValueError(f"no 4-bit pages of {page_size} tokens, {kv_heads} heads of {head_dim}: page_size is a multiple of 16, "
+                         "head_dim 32, 64 or 128")
     return torch.zeros(num_pages, kv_heads, page_size // 16, 20 * head_dim, dtype=torch.uint8, device=device)
 
 
 def _cache(pages, block_table):
-    _need(isinstance(pages, torch.Tensor) and pages.is_cuda, "pages must be a tensor on the GPU (see kv4_pages)")
-    _check("pages", pages, pages.device, (torch.uint8,), 4)
+    """(the cache's description, its GPU)."""
+    if not isinstance(pages, _Tensor) or not pages.is_cuda:
+        raise ValueError("pages must be a tensor on the GPU (see kv4_pages)")
+    index = pages.get_device()
+    _check("pages", pages, index, _U8, 4)
     n, heads, blocks, width = pages.shape
-    _need(width in (640, 1280, 2560) and pages.is_contiguous() and pages.numel() > 0,
-          "pages must be contiguous [num_pages, kv_heads, page_size / 16, 20 * head_dim] with head_dim 32, 64 or 128")
-    _check("block_table", block_table, pages.device, (torch.int32,), 2)
+    if width not in (640, 1280, 2560) or not pages.is_contiguous() or n * heads * blocks == 0:
+        raise ValueError("pages must be contiguous [num_pages, kv_heads, page_size / 16, 20 * head_dim] with head_dim 32, 64 or 128")
+    _check("block_table", block_table, index, _I32, 2)
     seqs, wide = block_table.shape
-    _need(wide > 0 and (wide == 1 or block_table.stride(1) == 1), "block_table must be [seqs, pages] with contiguous rows")
-    stride = block_table.stride(0) if seqs > 1 else wide
-    _need(stride >= wide, "block_table rows must not overlap")
-    return L.Kv4Cache(pages.data_ptr(), n, 16 * blocks, heads, width // 20, seqs, block_table.data_ptr(), stride, wide)
+    stride, step = block_table.stride()
+    if seqs <= 1:
+        stride = wide
+    if wide == 0 or wide > 1 and step != 1 or stride < wide:
+        raise ValueError("block_table must be [seqs, pages] with contiguous rows that do not overlap")
+    return L.Kv4Cache(pages.data_ptr(), n, 16 * blocks, heads, width // 20, seqs, block_table.data_ptr(), stride, wide), index
 
 
 def rope_table(rot_dim, positions, base=10000.0, factor=1.0, device="cuda"):
     """(cos, sin) of the angles position / factor * base^(-2 i / rot_dim): f32 [positions, rot_dim / 2, 2], formed in 64
     bits. `factor` > 1 squeezes a longer context into the trained one (linear position interpolation); a larger `base` is
     the other usual way of scaling."""
-    _need(rot_dim > 0 and rot_dim % 2 == 0 and positions > 0 and factor > 0 and base > 0,
-          "rope_table needs an even rot_dim and positive positions, base and factor")
+    if rot_dim <= 0 or rot_dim % 2 != 0 or positions <= 0 or factor <= 0 or base <= 0:
+        raise ValueError("rope_table needs an even rot_dim and positive positions, base and factor")
     angle = torch.arange(positions, dtype=torch.float64)[:, None] / factor * base ** (
         -torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
     return torch.stack([angle.cos(), angle.sin()], -1).float().to(device)
@@ -115,36 +129,38 @@ def kv4_append(pages, k, v, block_table, starts, cu_tokens=None, q=None, rope=No
     left alone); None: one new token per sequence. rope: a `rope_table`; keys and `q` [tokens, heads, head_dim] are rotated
     at their cache index, in halves or interleaved pairs, the first rot_dim dims of a head.
     Returns the rotated queries (a new tensor), q itself where there is nothing to rotate, None without q."""
-    cache = _cache(pages, block_table)
-    dev = pages.device
+    cache, dev = _cache(pages, block_table)
+    hd = cache.head_dim
     a = L.Kv4AppendArgs()
     a.cache = cache
-    a.k, a.k_token_stride, a.k_head_stride = _rows("k", k, dev, _HALF, cache.kv_heads, cache.head_dim)
-    a.v, a.v_token_stride, a.v_head_stride = _rows("v", v, dev, (k.dtype,), cache.kv_heads, cache.head_dim)
-    a.tokens = k.shape[0]
-    _need(v.shape[0] == k.shape[0], "k and v must have the same number of tokens")
-    a.dtype = _DTYPE[k.dtype]
-    a.starts = _ints("starts", starts, dev, cache.seqs)
+    a.k, a.k_token_stride, a.k_head_stride = _rows("k", k, dev, _HALF, cache.kv_heads, hd)
+    dtype, tokens = k.dtype, k.shape[0]
+    a.v, a.v_token_stride, a.v_head_stride = _rows("v", v, dev, (dtype,), cache.kv_heads, hd)
+    a.tokens, a.dtype = tokens, _DTYPE[dtype]
+    if v.shape[0] != tokens or q is not None and q.shape[0] != tokens:
+        raise ValueError("q, k and v must have the same number of tokens")
+    a.starts = _vector("starts", starts, dev, cache.seqs)
     if cu_tokens is not None:
-        a.cu_tokens = _ints("cu_tokens", cu_tokens, dev, cache.seqs + 1)
-    else:
-        _need(k.shape[0] == cache.seqs, "without cu_tokens there is one token per sequence")
+        a.cu_tokens = _vector("cu_tokens", cu_tokens, dev, cache.seqs + 1)
+    elif tokens != cache.seqs:
+        raise ValueError("without cu_tokens there is one token per sequence")
     out = q
     if q is not None:
-        q_rows = _rows("q", q, dev, (k.dtype,), None, cache.head_dim)
-        _need(q.shape[0] == k.shape[0], "q and k must have the same number of tokens")
+        q_rows = _rows("q", q, dev, (dtype,), None, hd)
     if rope is not None:
-        _check("rope", rope, dev, (torch.float32,), 3)
-        _need(rope.shape[2] == 2 and rope.is_contiguous() and 0 < 2 * rope.shape[1] <= cache.head_dim and rope.shape[0] > 0,
-              "rope must be a contiguous [positions, rot_dim / 2, 2] table with rot_dim <= head_dim (see rope_table)")
-        a.rope, a.rope_positions, a.rope_dim, a.rope_interleaved = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], int(interleaved)
-        if q is not None and q.numel() > 0:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _check("rope", rope, dev, _F32, 3)
+        positions, pairs, two = rope.shape
+        if two != 2 or not rope.is_contiguous() or not 0 < 2 * pairs <= hd or positions == 0:
+            raise ValueError("rope must be a contiguous [positions, rot_dim / 2, 2] table with rot_dim <= head_dim (see rope_table)")
+        a.rope, a.rope_positions, a.rope_dim, a.rope_interleaved = rope.data_ptr(), positions, 2 * pairs, int(interleaved)
+        if q is not None and q.shape[1]:
+            heads = q.shape[1]
+            out = torch.empty((tokens, heads, hd), dtype=dtype, device=q.device)
             a.q, a.q_token_stride, a.q_head_stride = q_rows
-            a.q_out, a.out_token_stride, a.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
-            a.heads = q.shape[1]
-    a.device_status = _status(status, dev)
-    if a.tokens:
+            a.q_out, a.out_token_stride, a.out_head_stride, a.heads = out.data_ptr(), heads * hd, hd, heads
+    if status is not None:
+        a.device_status = _status(status, dev)
+    if tokens:
         _call("crl_kv4_append", a, dev)
     return out
 
@@ -153,22 +169,27 @@ def kv4_read(pages, block_table, starts, tokens, cu_tokens=None, dtype=torch.flo
     """The keys and values that the cache holds, [tokens, kv_heads, head_dim] each in `dtype` (f16 or bf16): row
     cu_tokens[s] + j is cache index starts[s] + j of sequence s (without cu_tokens: row s is index starts[s]). Rows behind
     the last sequence, and rows without a page, are zero."""
-    cache = _cache(pages, block_table)
-    dev = pages.device
-    _need(dtype in _HALF, "kv4_read gives float16 or bfloat16")
-    k = torch.zeros(tokens, cache.kv_heads, cache.head_dim, dtype=dtype, device=dev)
-    v = torch.zeros_like(k)
+    cache, dev = _cache(pages, block_table)
+    if dtype not in _HALF:
+        raise ValueError("kv4_read gives float16 or bfloat16")
+    heads, hd = cache.kv_heads, cache.head_dim
+    k = torch.empty((tokens, heads, hd), dtype=dtype, device=pages.device)
+    v = torch.empty((tokens, heads, hd), dtype=dtype, device=pages.device)
     a = L.Kv4ReadArgs()
     a.cache, a.dtype, a.tokens = cache, _DTYPE[dtype], tokens
-    a.k, a.k_token_stride, a.k_head_stride = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.v_token_stride, a.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
-    a.starts = _ints("starts", starts, dev, cache.seqs)
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_token_stride = a.v_token_stride = heads * hd
+    a.k_head_stride = a.v_head_stride = hd
+    a.starts = _vector("starts", starts, dev, cache.seqs)
     if cu_tokens is not None:
-        a.cu_tokens = _ints("cu_tokens", cu_tokens, dev, cache.seqs + 1)
-    else:
-        _need(tokens == cache.seqs, "without cu_tokens there is one token per sequence")
-    a.device_status = _status(status, dev)
+        a.cu_tokens = _vector("cu_tokens", cu_tokens, dev, cache.seqs + 1)
+    elif tokens != cache.seqs:
+        raise ValueError("without cu_tokens there is one token per sequence")
+    if status is not None:
+        a.device_status = _status(status, dev)
     if tokens:
+        if cache.seqs == 0:
+            return k.zero_(), v.zero_()
         _call("crl_kv4_read", a, dev)
     return k, v
 
@@ -180,29 +201,37 @@ def kv4_attention(pages, q, block_table, lengths, cu_tokens=None, max_tokens=1, 
     max_tokens the most new tokens of any sequence (it sizes the launch; a sequence with more has the rest left out and
     reported through `status`). heads is a multiple of the cache's kv_heads. scale defaults to head_dim ** -0.5. A row that
     sees nothing is zero; rows behind the last sequence are left as they were in `out` (undefined in a new tensor)."""
-    cache = _cache(pages, block_table)
-    dev = pages.device
+    cache, dev = _cache(pages, block_table)
+    hd = cache.head_dim
     a = L.Kv4AttentionArgs()
     a.cache = cache
-    a.q, a.q_token_stride, a.q_head_stride = _rows("q", q, dev, _HALF, None, cache.head_dim)
-    _need(q.shape[1] > 0 and q.shape[1] % cache.kv_heads == 0, f"query heads must be a multiple of the cache's {cache.kv_heads}")
+    a.q, a.q_token_stride, a.q_head_stride = _rows("q", q, dev, _HALF, None, hd)
+    tokens, heads, _ = q.shape
+    dtype = q.dtype
+    if heads == 0 or heads % cache.kv_heads != 0:
+        raise ValueError(f"query heads must be a multiple of the cache's {cache.kv_heads}, got {heads}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty((tokens, heads, hd), dtype=dtype, device=q.device)
+        a.out, a.out_token_stride, a.out_head_stride = out.data_ptr(), heads * hd, hd
     else:
-        _need(isinstance(out, torch.Tensor) and out.shape[0] == q.shape[0], "out must have q's shape")
-    a.out, a.out_token_stride, a.out_head_stride = _rows("out", out, dev, (q.dtype,), q.shape[1], cache.head_dim)
-    a.dtype, a.heads, a.tokens = _DTYPE[q.dtype], q.shape[1], q.shape[0]
-    a.lengths = _ints("lengths", lengths, dev, cache.seqs)
+        a.out, a.out_token_stride, a.out_head_stride = _rows("out", out, dev, (dtype,), heads, hd)
+        if out.shape[0] != tokens:
+            raise ValueError("out must have q's shape")
+    a.dtype, a.heads, a.tokens = _DTYPE[dtype], heads, tokens
+    a.lengths = _vector("lengths", lengths, dev, cache.seqs)
     if cu_tokens is not None:
-        a.cu_tokens = _ints("cu_tokens", cu_tokens, dev, cache.seqs + 1)
-        _need(max_tokens >= 1, "max_tokens must be at least 1")
-        a.max_tokens = min(max_tokens, q.shape[0])
+        a.cu_tokens = _vector("cu_tokens", cu_tokens, dev, cache.seqs + 1)
+        if max_tokens < 1:
+            raise ValueError("max_tokens must be at least 1")
+        a.max_tokens = min(max_tokens, tokens)
     else:
-        _need(q.shape[0] == cache.seqs, "without cu_tokens there is one token per sequence")
+        if tokens != cache.seqs:
+            raise ValueError("without cu_tokens there is one token per sequence")
         a.max_tokens = 1
-    a.scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-    a.device_status = _status(status, dev)
-    if q.shape[0]:
+    a.scale = hd ** -0.5 if scale is None else scale
+    if status is not None:
+        a.device_status = _status(status, dev)
+    if tokens:
         _call("crl_kv4_attention", a, dev)
     return out
 
@@ -218,61 +247,65 @@ def adjust_logits(logits, history=None, repetition=None, frequency=None, presenc
     bitsets as positions.legal_mask_1929 and Engine.legal_masks make them); mask_rows int32 [rows] says which mask a row
     takes (negative: none), without it row r takes mask r. fp32 inside, rounded once. Returns `out` (a new tensor unless
     given; it may be `logits`)."""
-    _need(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be a tensor on the GPU")
-    dev = logits.device
-    _check("logits", logits, dev, tuple(_DTYPE), 2)
+    if not isinstance(logits, _Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a tensor on the GPU")
+    dev = logits.get_device()
+    _check("logits", logits, dev, _ANY, 2)
     rows, vocab = logits.shape
-    _need(vocab > 0, "logits must have a vocabulary")
+    if vocab == 0:
+        raise ValueError("logits must have a vocabulary")
     a = L.LogitsArgs()
 
-    def pitch(name, t):
-        _need(t.shape[1] <= 1 or t.stride(1) == 1, f"the rows of {name} must be contiguous")
-        stride = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-        _need(stride >= t.shape[1], f"the rows of {name} must not overlap")
-        return t.data_ptr(), stride
-
-    def per_row(name, t):
-        _check(name, t, dev, (torch.float32,), 1)
-        _need(t.shape[0] == rows and (rows <= 1 or t.stride(0) == 1), f"{name} must hold {rows} contiguous float32")
-        return t.data_ptr()
+    def matrix(name, t, dtypes, count):
+        """(address, elements from row to row, columns) of a matrix of `count` rows."""
+        _check(name, t, dev, dtypes, 2)
+        (n, wide), (stride, step) = t.shape, t.stride()
+        if n != count and count is not None:
+            raise ValueError(f"{name} must have {count} rows, got shape {tuple(t.shape)}")
+        if n <= 1:
+            stride = wide
+        if wide > 1 and step != 1 or stride < wide:
+            raise ValueError(f"the rows of {name} must be contiguous and not overlap")
+        return t.data_ptr(), stride, wide
 
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    _check("out", out, dev, (logits.dtype,), 2)
-    _need(out.shape == logits.shape, "out must have the shape of logits")
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        a.out, a.out_stride = out.data_ptr(), vocab
+    else:
+        a.out, a.out_stride, wide = matrix("out", out, (logits.dtype,), rows)
+        if wide != vocab:
+            raise ValueError("out must have the shape of logits")
     a.dtype, a.vocab, a.rows = _DTYPE[logits.dtype], vocab, rows
-    pointer, a.in_stride = pitch("logits", logits)
-    setattr(a, "in", pointer)
-    a.out, a.out_stride = pitch("out", out)
+    a.logits, a.in_stride, _ = matrix("logits", logits, _ANY, rows)
     if history is not None:
-        _check("history", history, dev, (torch.int32,), 2)
-        _need(history.shape[0] == rows, f"history must have {rows} rows")
-        a.history, a.history_stride = pitch("history", history)
-        a.history_len = history.shape[1]
-    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-        if t is not None:
-            setattr(a, name, per_row(name, t))
-    _need((bias_ids is None) == (bias_values is None), "bias_ids and bias_values go together")
-    if bias_ids is not None:
-        _check("bias_ids", bias_ids, dev, (torch.int32,), 2)
-        _check("bias_values", bias_values, dev, (torch.float32,), 2)
-        _need(bias_ids.shape[0] == rows and bias_ids.shape == bias_values.shape, f"bias_ids and bias_values must be [{rows}, m] both")
-        a.bias_ids, a.bias_stride = pitch("bias_ids", bias_ids)
-        a.bias_values, a.value_stride = pitch("bias_values", bias_values)
-        a.biases = bias_ids.shape[1]
-    _need(mask is not None or mask_rows is None, "mask_rows needs a mask")
+        a.history, a.history_stride, a.history_len = matrix("history", history, _I32, rows)
+    if repetition is not None:
+        a.repetition = _vector("repetition", repetition, dev, rows, _F32)
+    if frequency is not None:
+        a.frequency = _vector("frequency", frequency, dev, rows, _F32)
+    if presence is not None:
+        a.presence = _vector("presence", presence, dev, rows, _F32)
+    if bias_ids is not None or bias_values is not None:
+        if bias_ids is None or bias_values is None:
+            raise ValueError("bias_ids and bias_values go together")
+        a.bias_ids, a.bias_stride, a.biases = matrix("bias_ids", bias_ids, _I32, rows)
+        a.bias_values, a.value_stride, wide = matrix("bias_values", bias_values, _F32, rows)
+        if wide != a.biases:
+            raise ValueError("bias_ids and bias_values must have the same shape")
     if mask is not None:
-        _check("mask", mask, dev, (torch.uint8,), 2)
-        _need(mask.shape[1] * 8 >= vocab, f"mask rows hold {mask.shape[1]} bytes, the vocabulary needs {(vocab + 7) // 8}")
-        _need(mask.shape[0] > 0 or rows == 0, "mask must have a row")
-        a.mask, a.mask_stride = pitch("mask", mask)
+        a.mask, a.mask_stride, wide = matrix("mask", mask, _U8, rows if mask_rows is None else None)
         a.mask_count = mask.shape[0]
+        if wide * 8 < vocab:
+            raise ValueError(f"mask rows hold {wide} bytes, the vocabulary needs {(vocab + 7) // 8}")
+        if a.mask_count == 0 and rows:
+            raise ValueError("mask must have a row")
         if mask_rows is not None:
-            a.mask_rows = _ints("mask_rows", mask_rows, dev, rows)
-        else:
-            _need(mask.shape[0] == rows, f"mask must have {rows} rows, or mask_rows must say which one a row takes")
-    a.masked_value = float(masked_value)
-    a.device_status = _status(status, dev)
+            a.mask_rows = _vector("mask_rows", mask_rows, dev, rows)
+    elif mask_rows is not None:
+        raise ValueError("mask_rows needs a mask")
+    a.masked_value = masked_value
+    if status is not None:
+        a.device_status = _status(status, dev)
     if rows:
         _call("crl_adjust_logits", a, dev)
     return out

@@ -335,7 +335,8 @@ typedef struct crl_kv4_append_args {
 } crl_kv4_append_args;
 int crl_kv4_append(const crl_kv4_append_args* args);
 
-/* The values that the cache holds for the same rows (cache indices starts[s] + j), rounded to `dtype`. */
+/* The values that the cache holds for the same rows (cache indices starts[s] + j), rounded to `dtype`; rows behind the
+ * last sequence and rows without a page are zero. */
 typedef struct crl_kv4_read_args {
   crl_kv4_cache cache;
   int32_t dtype;
@@ -368,16 +369,16 @@ typedef struct crl_kv4_attention_args {
 } crl_kv4_attention_args;
 int crl_kv4_attention(const crl_kv4_attention_args* args);
 
-/* Next-token logits before a move is drawn from them: with z = in[row, v] and n = how often v stands in the row's history
+/* Next-token logits before a move is drawn from them: with z = logits[row, v] and n = how often v stands in the row's history
  *   n > 0: z = (z > 0 ? z / repetition : z * repetition) - (frequency * n + presence);   z += bias of v;
  *   bit v of the row's mask clear: z = masked_value.
  * fp32, each operation rounded once. The bitsets are those of crl_legal_mask_1929 / crl_legal_masks_packed104. Entries of
- * history and bias_ids outside the vocabulary are padding; of equal bias ids in a row the last one counts. out may be in. */
+ * history and bias_ids outside the vocabulary are padding; of equal bias ids in a row the last one counts. out may be logits. */
 typedef struct crl_logits_args {
-  int32_t dtype;               /* CRL_OUT_F32 / CRL_OUT_F16 / CRL_OUT_BF16 of in and out */
+  int32_t dtype;               /* CRL_OUT_F32 / CRL_OUT_F16 / CRL_OUT_BF16 of logits and out */
   int32_t vocab;
   int64_t rows;
-  const void* in; int64_t in_stride;
+  const void* logits; int64_t in_stride;
   void* out; int64_t out_stride;
   const int32_t* history; int64_t history_stride; int32_t history_len;   /* [rows, history_len], up to 2^20 - 1 */
   const float* repetition;     /* nullable, [rows]; default 1 */

@@ -47,7 +47,7 @@ def test_refusals_reach_no_kernel(lib):
         assert lib.crl_kv4_append(ctypes.byref(L.Kv4AppendArgs(cache=cache(), **{**append, **change}))) == rc, change
     for change, rc in ((dict(q=None), -1), (dict(heads=3), -2), (dict(heads=0), -1), (dict(lengths=None), -1)):
         assert lib.crl_kv4_attention(ctypes.byref(L.Kv4AttentionArgs(cache=cache(), **{**attend, **change}))) == rc, change
-    logits = {"dtype": L.OUT_F32, "vocab": 8, "rows": 2, "in": p, "in_stride": 8, "out": p, "out_stride": 8}
+    logits = {"dtype": L.OUT_F32, "vocab": 8, "rows": 2, "logits": p, "in_stride": 8, "out": p, "out_stride": 8}
     for change, rc in ((dict(vocab=0), -1), (dict(in_stride=7), -1), (dict(out_stride=7), -1), (dict(dtype=3), -1), (dict(out=None), -1),
                        (dict(history_len=3), -1), (dict(history_len=3, history=p, history_stride=2), -1),
                        (dict(history_len=1 << 20, history=p, history_stride=1 << 20), -2),
