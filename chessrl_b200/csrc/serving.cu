@@ -62,8 +62,15 @@ int current_sms(int* sms) {
   return CRL_OK;
 }
 
-int grid_of(int64_t rows, int hd, unsigned* grid) {
-  const int64_t blocks = (rows * (hd / 8) + 255) / 256;
+// Tokens of a CTA and the grid for `rows` rows per token: few tokens get a CTA each, many share the look-up of theirs.
+template <typename P>
+int by_tokens(P* p, int64_t rows, unsigned* grid) {
+  int sms = 0;
+  if (const int rc = current_sms(&sms)) return rc;
+  if (rows > 16384) return CRL_ERR_SHAPE;      // over_rows divides exactly up to here
+  p->per_cta = static_cast<int32_t>(std::min<int64_t>(kKv4CtaTokens, std::max<int64_t>(1, p->tokens / (8 * sms))));
+  p->over_rows = static_cast<uint32_t>(((uint64_t{1} << 32) + rows - 1) / rows);
+  const int64_t blocks = (p->tokens + p->per_cta - 1) / p->per_cta;
   if (blocks > INT32_MAX) return CRL_ERR_SHAPE;
   *grid = static_cast<unsigned>(blocks);
   return CRL_OK;
@@ -71,19 +78,19 @@ int grid_of(int64_t rows, int hd, unsigned* grid) {
 
 template <typename T, int HD>
 struct Append {
-  static int run(const Kv4AppendParams& p, cudaStream_t s) {
+  static int run(Kv4AppendParams p, cudaStream_t s) {
     unsigned grid;
-    if (grid_of(p.tokens * (p.heads + 2 * p.kv_heads), HD, &grid) != CRL_OK) return CRL_ERR_SHAPE;
-    kv4_append_kernel<T, HD><<<grid, 256, 0, s>>>(p);
+    if (const int rc = by_tokens(&p, static_cast<int64_t>(p.heads) + 2 * p.kv_heads, &grid)) return rc;
+    kv4_append_kernel<T, HD><<<grid, kKv4Threads, 0, s>>>(p);
     return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
   }
 };
 template <typename T, int HD>
 struct Read {
-  static int run(const Kv4ReadParams& p, cudaStream_t s) {
+  static int run(Kv4ReadParams p, cudaStream_t s) {
     unsigned grid;
-    if (grid_of(p.tokens * 2 * p.kv_heads, HD, &grid) != CRL_OK) return CRL_ERR_SHAPE;
-    kv4_read_kernel<T, HD><<<grid, 256, 0, s>>>(p);
+    if (const int rc = by_tokens(&p, int64_t{2} * p.kv_heads, &grid)) return rc;
+    kv4_read_kernel<T, HD><<<grid, kKv4Threads, 0, s>>>(p);
     return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
   }
 };
