@@ -46,10 +46,11 @@ struct Kv4Table {
   int64_t stride;
   int32_t width;          // pages a sequence can have
   int32_t blocks;         // 16-token blocks per page
+  int32_t shift;          // its logarithm where it is a power of two, else -1
   int64_t num_pages;
 };
 __device__ __forceinline__ int64_t kv4_block_of(const Kv4Table& t, int kv_heads, int seq, int block) {
-  const int slot = block / t.blocks;
+  const int slot = t.shift >= 0 ? block >> t.shift : block / t.blocks;
   if (block < 0 || slot >= t.width) return -1;
   const int64_t page = t.table[static_cast<int64_t>(seq) * t.stride + slot];
   if (page < 0 || page >= t.num_pages) return -1;

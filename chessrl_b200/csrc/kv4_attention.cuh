@@ -12,11 +12,11 @@
 //   exact operands for one logical instruction per two codes. The factor 16 of every other pair is taken out of q
 //   beforehand (scores) or out of the result (output); the offset 8 is the accumulator's start (scores) or comes out
 //   of one more product with a constant operand (output).
-// Scores: S = sum over groups of s_k * (q . (n - 8)) + c_k * sum(q), exact codes, q scaled to [1, 2) per row, fp32.
-// Output: P' = p * s rounded to f16 once, relative to the largest step seen so far (a power of two R per group), times the
-// codes; the centres' share p * c is summed in fp32. The products with n and with the offset 8 share the rounded P', so
-// its rounding weighs on the centred codes only.
-//
+// Scores: S = sum over groups of s_k * (q . n) + (c_k - 8 s_k) * sum(q), exact codes, q scaled to [1, 2) per row, fp32.
+// Output: P' = p * s rounded to f16 once, times the codes; the centres' share p * c is summed in fp32. The products with n
+// and with the offset 8 share the rounded P', so its rounding weighs on the centred codes only. p runs up to 8 (the
+// maximum is taken 3 higher in log2; the sum carries the same factor): P' stays below 8 * 7648 < 65504 whatever the steps,
+// and is a normal f16 number, with its full eleven bits, down to p s = 2^-17 of the largest p.
 // Bound by memory: 20 hd bytes per 16 cached tokens and key head, brought in by one bulk copy per block into a ring that
 // belongs to the warp (no barrier among warps before the join).
 #pragma once
@@ -55,6 +55,13 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d = a b, without an accumulator to clear
+__device__ __forceinline__ void mma_f16_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -83,20 +90,22 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {
   else { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
 }
 
-template <int HD, int NT, int WARPS, int STAGES>
+template <int HD, int NT, int WARPS>
 struct Kv4AttnShape {
-  static constexpr int kTile = 4;                                  // blocks of a tile
+  static constexpr int kTile = HD == 128 ? 2 : 4;                  // blocks of a tile: as many as 128 registers allow
+  static constexpr int kStages = HD == 32 ? 4 : 2;               // about 160 KB of an SM's shared memory for its 16 warps
   static constexpr int kStage = kTile * kv4_block_bytes(HD);
   static constexpr int kRows = 8 * NT;
-  static constexpr int kRing = WARPS * STAGES * kStage;
+  static constexpr int kRing = WARPS * kStages * kStage;
   static constexpr int kPart = kRows * (HD + 2) * 4;               // a warp's output, maximum and sum
   static constexpr int kJoin = (WARPS + 1) * kPart;                // the warps' and the CTA's
-  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + WARPS * STAGES * 8;
+  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + WARPS * kStages * 8;
 };
 
-template <typename T, int HD, int NT, int WARPS, int STAGES>
-__global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4AttentionParams p) {
-  using Shape = Kv4AttnShape<HD, NT, WARPS, STAGES>;
+template <typename T, int HD, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) kv4_attention_kernel(const Kv4AttentionParams p) {
+  using Shape = Kv4AttnShape<HD, NT, WARPS>;
+  constexpr int STAGES = Shape::kStages, KEYS = 16 * Shape::kTile, ALL = (1 << Shape::kTile) - 1;
   constexpr int G = HD / 32, MT = HD / 16, BB = kv4_block_bytes(HD), TB = Shape::kTile, ROWS = Shape::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -126,7 +135,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
   const int first_tok = row0 / p.group;
   const int seen_most = max(0, min(len, len - run + last_tok + 1));
   const int seen_least = max(0, min(len, len - run + first_tok + 1));
-  const int tiles = (seen_most + 64 - 1) / 64, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
+  const int tiles = (seen_most + KEYS - 1) / KEYS, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
 
   if (lane < STAGES) mbar_init(bars + lane * 8, 1);
   mbar_fence_init();
@@ -134,14 +143,15 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
 
   const int first = rank * WARPS + warp, step = splits * WARPS;
   uint32_t held = 0;      // four bits per stage: which blocks of the tile are there
-  auto issue = [&](int tile, int stage) {
-    const int nb = min(TB, blocks - tile * TB);
-    int64_t at = -1;
-    if (lane < nb) {
-      at = kv4_block_of(p.table, p.kv_heads, seq, tile * TB + lane);
-      if (at < 0) kv4_report(p.status, kDevKv4Table);
-    }
-    const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & 15u;
+  // lane b looks block b of a tile up (well before it is wanted: the table lies in global memory) and copies it
+  auto look_up = [&](int tile) -> int64_t {
+    if (lane >= min(TB, blocks - tile * TB)) return -1;
+    const int64_t at = kv4_block_of(p.table, p.kv_heads, seq, tile * TB + lane);
+    if (at < 0) kv4_report(p.status, kDevKv4Table);
+    return at;
+  };
+  auto issue = [&](int64_t at, int stage) {
+    const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & ALL;
     if (lane == 0) mbar_expect_tx(bars + stage * 8, __popc(there) * BB);
     __syncwarp();
     if (at >= 0)
@@ -151,12 +161,12 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
   };
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
-    if (first + s * step < tiles) issue(first + s * step, s);
+    if (first + s * step < tiles) issue(look_up(first + s * step), s);
 
   // queries as the B operand: column r of n-tile j, scaled to [1, 2) by a power of two; nibbles 1, 3, 5, 7 of a word come
   // 16 times too large
   uint32_t qf[NT][G][4];
-  float start[NT][2][G], kcol[NT][2];      // per column 2t, 2t + 1: -8 sum(q) * 2^-24 per group and the factor of S
+  float qsum[NT][2][G], kcol[NT][2];      // per column 2t, 2t + 1: sum(q) * 2^-24 per group and the factor of S, >= 0
   int limit[NT][2];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -177,7 +187,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
     // exponent of the largest; 100 bounds the factors below (2^(24 + 100) is a finite fp32)
     const int e = big > 0.0f ? min(100, max(-100, static_cast<int>(__float_as_uint(big) >> 23) - 127)) : 0;
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    // a negative scale is taken into q, so that the largest score is the largest product
+    const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.scale_log2);
     float sums[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -194,7 +205,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
       sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
       sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
     }
-    const float factor = __uint_as_float(static_cast<uint32_t>(127 + 24 + e) << 23) * p.scale_log2;
+    const float factor = __uint_as_float(static_cast<uint32_t>(127 + 24 + e) << 23) * fabsf(p.scale_log2);
     const int lim = live ? len - run + tok + 1 : 0;
     // lane (r, t) needs columns 2t and 2t + 1: lanes 4 * (2t) and 4 * (2t + 1) hold them
 #pragma unroll
@@ -203,11 +214,12 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
       kcol[j][c] = __shfl_sync(0xffffffffu, factor, from);
       limit[j][c] = __shfl_sync(0xffffffffu, lim, from);
 #pragma unroll
-      for (int g = 0; g < G; ++g) start[j][c][g] = __shfl_sync(0xffffffffu, sums[g], from) * (-8.0f / 16777216.0f);
+      for (int g = 0; g < G; ++g) qsum[j][c][g] = __shfl_sync(0xffffffffu, sums[g], from) * (1.0f / 16777216.0f);
     }
   }
 
-  float acc[NT][MT][4], ones[NT][G][4], centre[NT][G][2], top[NT][2], sum[NT][2], norm[G], stepmax[G];
+  // ones: -8 sum(P') of groups 2i (elements 0, 1) and 2i + 1 (2, 3)
+  float acc[NT][MT][4], ones[NT][(G + 1) / 2][4], centre[NT][G][2], top[NT][2], sum[NT][2];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -216,17 +228,12 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
       for (int i = 0; i < 4; ++i) acc[j][m][i] = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ones[j][g][i] = 0.0f;
+      ones[j][g / 2][2 * (g & 1)] = ones[j][g / 2][2 * (g & 1) + 1] = 0.0f;
+      if (G == 1) ones[j][0][2] = ones[j][0][3] = 0.0f;
       centre[j][g][0] = centre[j][g][1] = 0.0f;
     }
     top[j][0] = top[j][1] = -INFINITY;
     sum[j][0] = sum[j][1] = 0.0f;
-  }
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    norm[g] = 1.0f;
-    stepmax[g] = 0.0f;
   }
 
   const int kr = (r >> 1) + 4 * (r & 1);      // row of a block that operand row r stands for; r + 8: kr + 8
@@ -250,28 +257,22 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
       for (int g = 0; g < G; ++g) {
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&m0[g]));
         const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&m1[g]));
-        const float ca = a.y * -0.125f, cc = c.y * -0.125f;     // start = -8 sum(q) 2^-24, so c * sum(q) 2^-24 = start * c / -8
+        const float ca = fmaf(-8.0f, a.x, a.y), cc = fmaf(-8.0f, c.x, c.y);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          float d[4] = {start[j][0][g], start[j][1][g], start[j][0][g], start[j][1][g]};
-          mma_f16_16816(d, w0[g] & 0x000f000fu, w1[g] & 0x000f000fu, w0[g] & 0x00f000f0u, w1[g] & 0x00f000f0u, qf[j][g][0], qf[j][g][1]);
+          float d[4];
+          mma_f16_16816_first(d, w0[g] & 0x000f000fu, w1[g] & 0x000f000fu, w0[g] & 0x00f000f0u, w1[g] & 0x00f000f0u, qf[j][g][0], qf[j][g][1]);
           mma_f16_16816(d, (w0[g] >> 8) & 0x000f000fu, (w1[g] >> 8) & 0x000f000fu, (w0[g] >> 8) & 0x00f000f0u,
                         (w1[g] >> 8) & 0x00f000f0u, qf[j][g][2], qf[j][g][3]);
-          if (g == 0) {
-            sc[b][j][0] = fmaf(ca, start[j][0][g], a.x * d[0]);
-            sc[b][j][1] = fmaf(ca, start[j][1][g], a.x * d[1]);
-            sc[b][j][2] = fmaf(cc, start[j][0][g], c.x * d[2]);
-            sc[b][j][3] = fmaf(cc, start[j][1][g], c.x * d[3]);
-          } else {
-            sc[b][j][0] = fmaf(ca, start[j][0][g], fmaf(a.x, d[0], sc[b][j][0]));
-            sc[b][j][1] = fmaf(ca, start[j][1][g], fmaf(a.x, d[1], sc[b][j][1]));
-            sc[b][j][2] = fmaf(cc, start[j][0][g], fmaf(c.x, d[2], sc[b][j][2]));
-            sc[b][j][3] = fmaf(cc, start[j][1][g], fmaf(c.x, d[3], sc[b][j][3]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float s = i < 2 ? a.x : c.x, o = (i < 2 ? ca : cc) * qsum[j][i & 1][g];
+            sc[b][j][i] = fmaf(s, d[i], g == 0 ? o : fmaf(i < 2 ? ca : cc, qsum[j][i & 1][g], sc[b][j][i]));
           }
         }
       }
     }
-    const uint32_t there = (held >> (4 * stage)) & 15u;
+    const uint32_t there = (held >> (4 * stage)) & ALL;
     // running maximum per column
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -280,20 +281,18 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
       for (int b = 0; b < TB; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float x = sc[b][j][i] * kcol[j][i & 1];
           if (MASKED) {
-            const int key = tile * 64 + b * 16 + kr + (i >> 1) * 8;
-            if (key >= limit[j][i & 1] || !((there >> b) & 1u)) x = -INFINITY;
+            const int key = tile * KEYS + b * 16 + kr + (i >> 1) * 8;
+            if (key >= limit[j][i & 1] || !((there >> b) & 1u)) sc[b][j][i] = -INFINITY;
           }
-          sc[b][j][i] = x;
-          most[i & 1] = fmaxf(most[i & 1], x);
+          most[i & 1] = fmaxf(most[i & 1], sc[b][j][i]);
         }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int m = 4; m < 32; m <<= 1) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], m));
-        const float now = fmaxf(top[j][c], most[c]);
-        most[c] = now;
+        // the maximum in log2 units, less 3; a hidden row's stays at minus infinity whatever its factor
+        most[c] = fmaxf(top[j][c], most[c] == -INFINITY ? -INFINITY : fmaf(most[c], kcol[j][c], -3.0f));
       }
       if (__any_sync(0xffffffffu, most[0] > top[j][0] || most[1] > top[j][1])) {
         float alpha[2];
@@ -310,93 +309,50 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
 #pragma unroll
         for (int g = 0; g < G; ++g) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ones[j][g][i] *= alpha[i & 1];
+          for (int c = 0; c < 2; ++c) ones[j][g / 2][2 * (g & 1) + c] *= alpha[c];
           centre[j][g][0] *= alpha[0];
           centre[j][g][1] *= alpha[1];
         }
       }
+      const float off[2] = {top[j][0] == -INFINITY ? 0.0f : top[j][0], top[j][1] == -INFINITY ? 0.0f : top[j][1]};
 #pragma unroll
       for (int b = 0; b < TB; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float off = top[j][i & 1] == -INFINITY ? 0.0f : top[j][i & 1];
-          sc[b][j][i] = exp2_approx(sc[b][j][i] - off);
+          float x = fmaf(sc[b][j][i], kcol[j][i & 1], -off[i & 1]);
+          if (MASKED && sc[b][j][i] == -INFINITY) x = -INFINITY;      // also where the factor is zero
+          sc[b][j][i] = exp2_approx(x);
           sum[j][i & 1] += sc[b][j][i];
         }
-    }
-    // steps of the values: the tile's largest, per group
-    uint32_t v0[TB][G], v1[TB][G];
-    float big[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) big[g] = 0.0f;
-#pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      const uint8_t* blk = base + b * BB + 18 * HD;
-      lds_words<G>(v0[b], blk + kr * (G * 4));
-      lds_words<G>(v1[b], blk + (kr + 8) * (G * 4));
-      if (MASKED) {
-        const int key = tile * 64 + b * 16 + kr;
-        const bool lost = !((there >> b) & 1u);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          if (lost || key >= seen_most) v0[b][g] = 0u;
-          if (lost || key + 8 >= seen_most) v1[b][g] = 0u;
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        big[g] = fmaxf(big[g], fmaxf(__low2float(*reinterpret_cast<const __half2*>(&v0[b][g])),
-                                     __low2float(*reinterpret_cast<const __half2*>(&v1[b][g]))));
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (__any_sync(0xffffffffu, big[g] > stepmax[g])) {
-        float now = big[g];
-#pragma unroll
-        for (int m = 4; m < 32; m <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, m));
-        // the least power of two above it, and its reciprocal
-        const int e = min(120, static_cast<int>(__float_as_uint(now) >> 23) - 126);
-        stepmax[g] = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-        const float next = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        const float beta = next / norm[g];
-        norm[g] = next;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ones[j][g][i] *= beta;
-            acc[j][2 * g][i] *= beta;
-            acc[j][2 * g + 1][i] *= beta;
-          }
-        }
-      }
     }
     // output
 #pragma unroll
     for (int b = 0; b < TB; ++b) {
-      uint32_t pf[NT][G][2];
+      uint32_t pf[NT][G][2], v0[G], v1[G];
+      lds_words<G>(v0, base + b * BB + 18 * HD + kr * (G * 4));
+      lds_words<G>(v1, base + b * BB + 18 * HD + (kr + 8) * (G * 4));
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v0[b][g]));
-        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v1[b][g]));
-        const float sa = a.x * norm[g], sb = c.x * norm[g];
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v0[g]));
+        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v1[g]));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const float* x = sc[b][j];
-          float y[4] = {x[0] * sa, x[1] * sa, x[2] * sb, x[3] * sb};
-          float z[4] = {x[0] * a.y, x[1] * a.y, x[2] * c.y, x[3] * c.y};
+          float y[4] = {x[0] * a.x, x[1] * a.x, x[2] * c.x, x[3] * c.x};
+          float z[4] = {a.y, a.y, c.y, c.y};
           if (MASKED) {      // a hidden key's row may hold anything
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int key = tile * 64 + b * 16 + kr + (i >> 1) * 8;
-              if (key >= limit[j][i & 1]) y[i] = z[i] = 0.0f;
+              const int key = tile * KEYS + b * 16 + kr + (i >> 1) * 8;
+              if (key >= limit[j][i & 1] || !((there >> b) & 1u)) y[i] = z[i] = 0.0f;
             }
           }
-          centre[j][g][0] += z[0] + z[2];
-          centre[j][g][1] += z[1] + z[3];
+          centre[j][g][0] = fmaf(x[0], z[0], fmaf(x[2], z[2], centre[j][g][0]));
+          centre[j][g][1] = fmaf(x[1], z[1], fmaf(x[3], z[3], centre[j][g][1]));
           pf[j][g][0] = transpose_8x8(pack_f16(y[0], y[1]));
           pf[j][g][1] = transpose_8x8(pack_f16(y[2], y[3]));
-          mma_f16_16816(ones[j][g], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[j][g][0], pf[j][g][1]);
+          if (g & 1) mma_f16_16816(ones[j][g / 2], 0u, 0x80088008u, 0u, 0x80088008u, pf[j][g][0], pf[j][g][1]);
+          else mma_f16_16816(ones[j][g / 2], 0x80088008u, 0u, 0x80088008u, 0u, pf[j][g][0], pf[j][g][1]);
         }
       }
       const uint8_t* blk = base + b * BB + 10 * HD;
@@ -437,12 +393,14 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
 
   int stage = 0;
   for (int tile = first; tile < tiles; tile += step) {
+    const bool more = tile + STAGES * step < tiles;
+    const int64_t ahead = more ? look_up(tile + STAGES * step) : -1;
     if (!mbar_wait(bars + stage * 8, (phase >> stage) & 1u)) { fine = false; break; }
     phase ^= 1u << stage;
-    if (tile * 64 + 64 > seen_least || ((held >> (4 * stage)) & 15u) != 15u) consume(std::true_type{}, tile, stage);
+    if (tile * KEYS + KEYS > seen_least || ((held >> (4 * stage)) & ALL) != ALL) consume(std::true_type{}, tile, stage);
     else consume(std::false_type{}, tile, stage);
     __syncwarp();
-    if (tile + STAGES * step < tiles) issue(tile + STAGES * step, stage);
+    if (more) issue(ahead, stage);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   if (!fine) {      // give up; the copies still under way end before their shared memory is used for something else
@@ -453,6 +411,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
   // join the warps: each leaves (maximum, sum, output) per row; the ring is free once every warp is here
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem) + warp * (Shape::kPart / 4);
+  const int live = min(rows, ROWS);
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -468,6 +427,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
         for (int m = 4; m < 32; m <<= 1) ce[g] += __shfl_xor_sync(0xffffffffu, ce[g], m);
       }
       const int row = j * 8 + 2 * t + c;
+      if (row >= live) continue;
       if (r == 0) {
         // a NaN sum must survive the join even where no score was a number
         part[ROWS * HD + row] = s != s ? INFINITY : top[j][c];
@@ -476,16 +436,16 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int g = m / 2;
-        const float f = 16777216.0f / norm[g];
-        part[row * HD + 16 * m + r] = fmaf(acc[j][m][c] + ones[j][g][c], f, ce[g]);
-        part[row * HD + 16 * m + 8 + r] = fmaf(acc[j][m][c + 2] + ones[j][g][c + 2], f * 0.0625f, ce[g]);
+        const float eight = ones[j][g / 2][2 * (g & 1) + c];
+        part[row * HD + 16 * m + r] = fmaf(acc[j][m][c] + eight, 16777216.0f, ce[g]);
+        part[row * HD + 16 * m + 8 + r] = fmaf(fmaf(acc[j][m][c + 2], 0.0625f, eight), 16777216.0f, ce[g]);
       }
     }
   }
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(smem);
   float* mine = reinterpret_cast<float*>(smem) + WARPS * (Shape::kPart / 4);
-  for (int i = threadIdx.x; i < ROWS * HD; i += WARPS * 32) {
+  for (int i = threadIdx.x; i < live * HD; i += WARPS * 32) {
     const int row = i / HD;
     float most = -INFINITY;
 #pragma unroll
@@ -509,7 +469,6 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(const Kv4Atte
   __syncwarp();
   if (splits > 1) cluster_sync(); else __syncthreads();
   const uint32_t mine_at = smem_u32(mine);
-  const int live = min(rows, ROWS);
   for (int i = rank * WARPS * 32 + threadIdx.x; i < live * HD; i += splits * WARPS * 32) {
     const int row = i / HD;
     float o, s;

@@ -22,7 +22,7 @@ struct Kv4RowsShape {
   static constexpr int kRing = KW * kStages * kStage;
   static constexpr int kPart = 16 * (HD + 2) * 4;
   static constexpr int kJoin = (RW * KW + RW) * kPart;
-  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + KW * kStages * 16;
+  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + KW * kStages * 20;
 };
 
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
@@ -47,7 +47,9 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   const int splits = gridDim.x, rank = blockIdx.x;
   const int head = blockIdx.y % p.kv_heads, row_tile = p.row_tiles - 1 - blockIdx.y / p.kv_heads, seq = blockIdx.z;
   uint8_t* ring = smem + kw * ST * Shape::kStage;
-  const uint32_t full = smem_u32(smem + Shape::kBytes - KW * ST * 16) + kw * ST * 16, empty = full + ST * 8;
+  const uint32_t full = smem_u32(smem + Shape::kBytes - KW * ST * 20) + kw * ST * 16, empty = full + ST * 8;
+  // which blocks of a stage's tile there are, left by the warp that copies them
+  uint32_t* held = reinterpret_cast<uint32_t*>(smem + Shape::kBytes - KW * ST * 4) + kw * ST;
 
   int len = p.lengths[seq];
   const int64_t q0 = p.cu != nullptr ? p.cu[seq] : seq;
@@ -68,7 +70,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   const int tiles = (seen_most + 63) / 64, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
 
   if (threadIdx.x < KW * ST) {
-    const uint32_t at = smem_u32(smem + Shape::kBytes - KW * ST * 16) + (threadIdx.x / ST) * ST * 16 + (threadIdx.x % ST) * 8;
+    const uint32_t at = smem_u32(smem + Shape::kBytes - KW * ST * 20) + (threadIdx.x / ST) * ST * 16 + (threadIdx.x % ST) * 8;
     mbar_init(at, 1);
     mbar_init(at + ST * 8, RW);
   }
@@ -76,16 +78,19 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   __syncthreads();
 
   const int first = rank * KW + kw, step = splits * KW;
-  // which blocks of a tile there are is worked out by every warp for itself (the copies are issued by the group's first)
-  auto block_at = [&](int tile) -> int64_t {
-    const int nb = min(4, blocks - tile * 4);
-    return lane < nb ? kv4_block_of(p.table, p.kv_heads, seq, tile * 4 + lane) : -1;
+  // lane b of a key group's first warp looks block b of a tile up (well before it is wanted) and copies it
+  auto look_up = [&](int tile) -> int64_t {
+    if (lane >= min(4, blocks - tile * 4)) return -1;
+    const int64_t at = kv4_block_of(p.table, p.kv_heads, seq, tile * 4 + lane);
+    if (at < 0) kv4_report(p.status, kDevKv4Table);
+    return at;
   };
-  auto issue = [&](int tile, int stage) {
-    const int64_t at = block_at(tile);
-    if (lane < min(4, blocks - tile * 4) && at < 0) kv4_report(p.status, kDevKv4Table);
+  auto issue = [&](int64_t at, int stage) {
     const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
-    if (lane == 0) mbar_expect_tx(full + stage * 8, __popc(there) * BB);
+    if (lane == 0) {
+      held[stage] = there;
+      mbar_expect_tx(full + stage * 8, __popc(there) * BB);
+    }
     __syncwarp();
     if (at >= 0)
       bulk_load(smem_u32(ring + stage * Shape::kStage + lane * BB),
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   if (rw == 0)
 #pragma unroll
     for (int s = 0; s < ST; ++s)
-      if (first + s * step < tiles) issue(first + s * step, s);
+      if (first + s * step < tiles) issue(look_up(first + s * step), s);
 
   // queries as the A operand, rows r and r + 8 of this warp, scaled to [1, 2) by a power of two
   uint32_t qf[G][2][4], qsum[2] = {0, 0};     // [group][half of the group][register]; sums: rows r, r + 8
@@ -317,17 +322,19 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   uint32_t phase = 0;
   bool fine = true;
   for (int tile = first; tile < tiles; tile += step) {
-    const uint32_t there = __ballot_sync(0xffffffffu, block_at(tile) >= 0);
+    const bool more = rw == 0 && tile + ST * step < tiles;
+    const int64_t ahead = more ? look_up(tile + ST * step) : -1;
     if (!mbar_wait(full + stage * 8, phase)) { fine = false; break; }
+    const uint32_t there = held[stage];
     if (tile * 64 < see_any) {
       if (tile * 64 + 64 > see_all || there != 15u) consume(std::true_type{}, tile, stage, there);
       else consume(std::false_type{}, tile, stage, there);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + stage * 8);
-    if (rw == 0 && tile + ST * step < tiles) {
+    if (more) {
       if (!mbar_wait(empty + stage * 8, phase)) { fine = false; break; }
-      issue(tile + ST * step, stage);
+      issue(ahead, stage);
     }
     if (++stage == ST) {
       stage = 0;

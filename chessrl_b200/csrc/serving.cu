@@ -36,6 +36,9 @@ Kv4Table table_of(const crl_kv4_cache& c) {
   t.stride = c.table_stride;
   t.width = c.table_width;
   t.blocks = c.page_size / kKv4Block;
+  t.shift = -1;
+  for (int b = 0; b < 30; ++b)
+    if (t.blocks == 1 << b) t.shift = b;
   t.num_pages = c.num_pages;
   return t;
 }
@@ -95,23 +98,69 @@ struct Read {
   }
 };
 
-// One launch of an attention kernel: a cluster of `splits` CTAs along the keys per (row tile, key head, sequence).
+constexpr int kMaxSplits = 8;      // the portable cluster size
+
+// What is known of an attention kernel on a device: how many clusters of 1 .. kMaxSplits CTAs are resident at once.
+struct KernelFacts {
+  std::atomic<int> clusters[kMaxSplits + 1];
+};
 template <typename K>
-int attend_launch(K* kernel, std::atomic<uint64_t>& ready, int bytes, int threads, int tile_rows, int keys_at_once, int resident,
-                  Kv4AttentionParams p, int sms, int64_t max_keys, cudaStream_t s) {
+int facts_of(K* kernel, KernelFacts* all, int bytes, int threads, KernelFacts** out) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return CRL_ERR_CUDA;
-  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
-  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {      // once per kernel and device
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return CRL_ERR_CUDA;
+  KernelFacts& f = all[dev];
+  if (f.clusters[0].load(std::memory_order_acquire) == 0) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return CRL_ERR_CUDA;
-    ready.fetch_or(bit, std::memory_order_relaxed);
+    for (int n = 1; n <= kMaxSplits; ++n) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(n);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = bytes;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = n;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      int many = 0;
+      if (cudaOccupancyMaxActiveClusters(&many, kernel, &cfg) != cudaSuccess) return CRL_ERR_CUDA;
+      f.clusters[n].store(many > 0 ? many : 1, std::memory_order_relaxed);
+    }
+    f.clusters[0].store(1, std::memory_order_release);
   }
+  *out = &f;
+  return CRL_OK;
+}
+
+// The number of CTAs that share the keys of a (row tile, key head, sequence): the one that makes the waves of clusters
+// times the key tiles of the longest warp least (`fixed` tiles' worth of time goes to a CTA's start and join), for
+// sequences as long as the table allows.
+int split_keys(const KernelFacts& f, int64_t units, int64_t max_keys, int keys_at_once, int fixed) {
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= kMaxSplits; ++n) {
+    const int64_t tiles = (max_keys + static_cast<int64_t>(n) * keys_at_once - 1) / (static_cast<int64_t>(n) * keys_at_once);
+    const int64_t active = f.clusters[n].load(std::memory_order_relaxed), waves = (units + active - 1) / active;
+    const int64_t cost = waves * (tiles + fixed + (n > 1 ? 1 : 0));
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+    if (tiles <= 1) break;
+  }
+  return best;
+}
+
+// One launch of an attention kernel: a cluster along the keys per (row tile, key head, sequence).
+template <typename K>
+int attend_launch(K* kernel, KernelFacts* all, int bytes, int threads, int tile_rows, int keys_at_once, Kv4AttentionParams p,
+                  int64_t max_keys, cudaStream_t s) {
+  KernelFacts* f = nullptr;
+  if (const int rc = facts_of(kernel, all, bytes, threads, &f)) return rc;
   p.row_tiles = (p.max_tokens * p.group + tile_rows - 1) / tile_rows;
   const int64_t units = static_cast<int64_t>(p.seqs) * p.kv_heads * p.row_tiles;
   if (static_cast<int64_t>(p.kv_heads) * p.row_tiles > 65535) return CRL_ERR_SHAPE;
-  // the axis of keys is split over a cluster while there are SMs without work and tiles for every warp
-  int splits = 1;
-  while (splits < 8 && units * splits * 2 <= resident * sms && static_cast<int64_t>(splits) * 2 * keys_at_once <= max_keys) splits *= 2;
+  const int splits = split_keys(*f, units, max_keys, keys_at_once, 2);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, p.kv_heads * p.row_tiles, p.seqs);
   cfg.blockDim = dim3(threads);
@@ -125,28 +174,32 @@ int attend_launch(K* kernel, std::atomic<uint64_t>& ready, int bytes, int thread
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const Kv4AttentionParams>(p)) == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
 }
-template <typename T, int HD>
-int attend_few(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
-  constexpr int WARPS = 8, STAGES = HD == 32 ? 3 : 2;
-  using Shape = Kv4AttnShape<HD, 1, WARPS, STAGES>;
-  static std::atomic<uint64_t> ready{0};
-  return attend_launch(kv4_attention_kernel<T, HD, 1, WARPS, STAGES>, ready, Shape::kBytes, WARPS * 32, Shape::kRows, WARPS * 64, 2, p,
-                       sms, max_keys, s);
+template <typename T, int HD, int WARPS>
+int attend_few(const Kv4AttentionParams& p, int64_t max_keys, cudaStream_t s) {
+  using Shape = Kv4AttnShape<HD, 1, WARPS>;
+  static KernelFacts facts[64];
+  return attend_launch(kv4_attention_kernel<T, HD, 1, WARPS>, facts, Shape::kBytes, WARPS * 32, Shape::kRows, WARPS * Shape::kTile * 16, p,
+                       max_keys, s);
 }
 template <typename T, int HD, int RW>
-int attend_rows(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
+int attend_rows(const Kv4AttentionParams& p, int64_t max_keys, cudaStream_t s) {
   using Shape = Kv4RowsShape<HD, RW, 4 / RW>;
-  static std::atomic<uint64_t> ready{0};
-  return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, ready, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, 2, p, sms, max_keys, s);
+  static KernelFacts facts[64];
+  return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, facts, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, p, max_keys, s);
 }
 template <typename T, int HD>
 struct Attend {
   static int run(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
     const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group;
-    if (rows <= 8) return attend_few<T, HD>(p, sms, max_keys, s);
-    if (rows <= 16) return attend_rows<T, HD, 1>(p, sms, max_keys, s);
-    if (rows <= 32) return attend_rows<T, HD, 2>(p, sms, max_keys, s);
-    return attend_rows<T, HD, 4>(p, sms, max_keys, s);
+    if (rows <= 8) {
+      // few (sequence, key head) pairs need more warps on each than eight CTAs of four
+      const int64_t units = static_cast<int64_t>(p.seqs) * p.kv_heads;
+      if (units * kMaxSplits < 4 * sms) return attend_few<T, HD, 8>(p, max_keys, s);
+      return attend_few<T, HD, 4>(p, max_keys, s);
+    }
+    if (rows <= 16) return attend_rows<T, HD, 1>(p, max_keys, s);
+    if (rows <= 32) return attend_rows<T, HD, 2>(p, max_keys, s);
+    return attend_rows<T, HD, 4>(p, max_keys, s);
   }
 };
 
