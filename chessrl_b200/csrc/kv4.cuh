@@ -40,21 +40,24 @@ __device__ __forceinline__ void kv4_report(int* status, int code) {
 }
 
 // Where the block of cache index `index` of a sequence lies: its number in [num_pages][kv_heads][blocks per page] for
-// head 0, or -1 for an index that the table does not cover or a page that the pool does not have.
+// head 0, or kNoBlock for an index that the table does not cover or a page that the pool does not have. Block numbers
+// are 32-bit (2^32 blocks of 640 bytes or more are more than a GPU holds; the host checks).
 struct Kv4Table {
   const int32_t* table;   // [seqs][stride]
   int64_t stride;
   int32_t width;          // pages a sequence can have
   int32_t blocks;         // 16-token blocks per page
   int32_t shift;          // its logarithm where it is a power of two, else -1
-  int64_t num_pages;
+  uint32_t num_pages;
+  uint32_t page_blocks;   // kv_heads * blocks
 };
-__device__ __forceinline__ int64_t kv4_block_of(const Kv4Table& t, int kv_heads, int seq, int block) {
+constexpr uint32_t kNoBlock = 0xffffffffu;
+__device__ __forceinline__ uint32_t kv4_block_of(const Kv4Table& t, const int32_t* row, int block) {
   const int slot = t.shift >= 0 ? block >> t.shift : block / t.blocks;
-  if (block < 0 || slot >= t.width) return -1;
-  const int64_t page = t.table[static_cast<int64_t>(seq) * t.stride + slot];
-  if (page < 0 || page >= t.num_pages) return -1;
-  return page * kv_heads * t.blocks + (block - slot * t.blocks);
+  if (static_cast<uint32_t>(slot) >= static_cast<uint32_t>(t.width)) return kNoBlock;
+  const uint32_t page = static_cast<uint32_t>(row[slot]);
+  if (page >= t.num_pages) return kNoBlock;
+  return page * t.page_blocks + static_cast<uint32_t>(block - slot * t.blocks);
 }
 
 // The sequence that token row `row` belongs to: the last one whose first row is not behind it (cu ascending, cu[0] = 0).
@@ -65,6 +68,15 @@ __device__ __forceinline__ int kv4_seq_of(const int32_t* cu, int seqs, int64_t r
     if (cu[mid] <= row) lo = mid; else hi = mid - 1;
   }
   return lo;
+}
+
+// n / d for a divisor that the host knows: one multiplication while n * d < 2^32
+struct Kv4Divisor {
+  uint32_t d, mul;      // mul = ceil(2^32 / d), 0 where the bound does not hold (or d is 1)
+};
+__device__ __forceinline__ int kv4_div(int n, const Kv4Divisor& v) {
+  if (v.mul != 0) return static_cast<int>(__umulhi(static_cast<uint32_t>(n), v.mul));
+  return v.d == 1 ? n : n / static_cast<int>(v.d);
 }
 
 template <typename T> __device__ __forceinline__ float kv4_to_float(T x);

@@ -71,7 +71,7 @@ __device__ __forceinline__ void kv4_rotate(const T* row, bool vec, const float2*
 constexpr int kKv4CtaTokens = 8, kKv4Threads = 256;
 
 struct Kv4Place {
-  int64_t block;      // block of head 0 that the token's row lies in, -1: none
+  uint32_t block;     // block of head 0 that the token's row lies in, kNoBlock: none
   int32_t row;        // its row there
   int32_t ok;         // the token belongs to a sequence (and has a place in the rotation table)
   const float2* rope;
@@ -80,7 +80,7 @@ struct Kv4Place {
 // Where the CTA's tokens go. Rows behind the last sequence have ok = 0.
 template <typename P>
 __device__ __forceinline__ Kv4Place kv4_place(const P& p, int64_t tok, const float2* rope, int64_t positions, int half) {
-  Kv4Place w{-1, 0, 0, nullptr};
+  Kv4Place w{kNoBlock, 0, 0, nullptr};
   if (tok >= p.tokens) return w;
   int seq = static_cast<int>(tok);
   int64_t offset = 0;
@@ -101,8 +101,9 @@ __device__ __forceinline__ Kv4Place kv4_place(const P& p, int64_t tok, const flo
   }
   w.ok = 1;
   w.row = static_cast<int32_t>(index & 15);
-  w.block = index < 0 || index > INT32_MAX ? -1 : kv4_block_of(p.table, p.kv_heads, seq, static_cast<int>(index >> 4));
-  if (w.block < 0) kv4_report(p.status, kDevKv4Table);
+  if (index >= 0 && index <= INT32_MAX)
+    w.block = kv4_block_of(p.table, p.table.table + seq * p.table.stride, static_cast<int>(index >> 4));
+  if (w.block == kNoBlock) kv4_report(p.status, kDevKv4Table);
   return w;
 }
 
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Append
       kv4_rotate(row, p.vec_q, w.rope, p.rot, p.interleaved, part, x);
       kv4_store8(static_cast<T*>(p.q_out) + tok * p.o_tok + h * p.o_head + part * 8, p.vec_o, x);
     }
-    const bool ok = live && !is_q && w.block >= 0;
+    const bool ok = live && !is_q && w.block != kNoBlock;
     if (!__any_sync(0xffffffffu, ok)) continue;
     h -= p.heads;
     const bool is_k = h < p.kv_heads;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Append
     uint32_t turned = transpose_nibbles(word, lane);
     if constexpr (HD == 32) turned = pair_rows(turned, lane);
     if (!ok) continue;
-    uint8_t* at = p.pages + (w.block + static_cast<int64_t>(h) * p.table.blocks) * kv4_block_bytes(HD) + (is_k ? 0 : 10 * HD);
+    uint8_t* at = p.pages + static_cast<size_t>(w.block + h * p.table.blocks) * kv4_block_bytes(HD) + (is_k ? 0 : 10 * HD);
     const int g = part / 4, t = part % 4;
     uint8_t* codes = at + w.row * (HD / 2);
     reinterpret_cast<uint32_t*>(codes)[is_k ? t * G + g : value_word<HD>(part)] = is_k ? word : turned;
@@ -247,8 +248,8 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const Kv4ReadPara
     const int64_t tok = tok0 + local;
     uint32_t word = 0;
     float s = 0.0f, c = 0.0f;      // a row that is not there is zero
-    if (w.block >= 0) {
-      const uint8_t* at = p.pages + (w.block + static_cast<int64_t>(h) * p.table.blocks) * kv4_block_bytes(HD) + (is_k ? 0 : 10 * HD);
+    if (w.block != kNoBlock) {
+      const uint8_t* at = p.pages + static_cast<size_t>(w.block + h * p.table.blocks) * kv4_block_bytes(HD) + (is_k ? 0 : 10 * HD);
       word = reinterpret_cast<const uint32_t*>(at + w.row * (HD / 2))[is_k ? t * G + g : value_word<HD>(part)];
       const float2 sc = __half22float2(reinterpret_cast<const __half2*>(at + 8 * HD + w.row * (HD / 8))[g]);
       s = sc.x;

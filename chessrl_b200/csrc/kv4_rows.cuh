@@ -44,8 +44,8 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int kw = warp / RW, rw = warp % RW;
-  const int splits = gridDim.x, rank = blockIdx.x;
-  const int head = blockIdx.y % p.kv_heads, row_tile = p.row_tiles - 1 - blockIdx.y / p.kv_heads, seq = blockIdx.z;
+  const int splits = cluster_size_x(), rank = cluster_ctarank();
+  const int head = blockIdx.y, row_tile = p.row_tiles - 1 - static_cast<int>(cluster_id_x()), seq = blockIdx.z;   // long rows first
   uint8_t* ring = smem + kw * ST * Shape::kStage;
   const uint32_t full = smem_u32(smem + Shape::kBytes - KW * ST * 20) + kw * ST * 16, empty = full + ST * 8;
   // which blocks of a stage's tile there are, left by the warp that copies them
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   }
   const int row0 = row_tile * ROWS, rows = run * p.group - row0;
   if (rows <= 0) return;      // the same for every CTA of the cluster
-  const int last_tok = min(row0 + ROWS - 1, run * p.group - 1) / p.group;
+  const int last_tok = kv4_div(min(row0 + ROWS - 1, run * p.group - 1), p.by_group);
   const int seen_most = max(0, min(len, len - run + last_tok + 1));
   const int tiles = (seen_most + 63) / 64, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
 
@@ -79,22 +79,24 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
 
   const int first = rank * KW + kw, step = splits * KW;
   // lane b of a key group's first warp looks block b of a tile up (well before it is wanted) and copies it
-  auto look_up = [&](int tile) -> int64_t {
-    if (lane >= min(4, blocks - tile * 4)) return -1;
-    const int64_t at = kv4_block_of(p.table, p.kv_heads, seq, tile * 4 + lane);
-    if (at < 0) kv4_report(p.status, kDevKv4Table);
+  const int32_t* pages_of = p.table.table + seq * p.table.stride;
+  const uint8_t* head_pages = p.pages + static_cast<size_t>(head) * p.table.blocks * BB;
+  auto look_up = [&](int tile) -> uint32_t {
+    if (lane >= min(4, blocks - tile * 4)) return kNoBlock;
+    const uint32_t at = kv4_block_of(p.table, pages_of, tile * 4 + lane);
+    if (at == kNoBlock) kv4_report(p.status, kDevKv4Table);
     return at;
   };
-  auto issue = [&](int64_t at, int stage) {
-    const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+  auto issue = [&](uint32_t at, int stage) {
+    const uint32_t there = __ballot_sync(0xffffffffu, at != kNoBlock);
     if (lane == 0) {
       held[stage] = there;
       mbar_expect_tx(full + stage * 8, __popc(there) * BB);
     }
     __syncwarp();
-    if (at >= 0)
+    if (at != kNoBlock)
       bulk_load(smem_u32(ring + stage * Shape::kStage + lane * BB),
-                p.pages + (at + static_cast<int64_t>(head) * p.table.blocks) * BB, BB, full + stage * 8);
+                head_pages + static_cast<size_t>(at) * BB, BB, full + stage * 8);
   };
   if (rw == 0)
 #pragma unroll
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   int limit[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int row = row0 + rw * 16 + r + 8 * h, tok = row / p.group;
+    const int row = row0 + rw * 16 + r + 8 * h, tok = kv4_div(row, p.by_group);
     const bool live = tok < run;
     const T* src = static_cast<const T*>(p.q) + (q0 + tok) * p.q_tok + static_cast<int64_t>(head * p.group + row - tok * p.group) * p.q_head;
     float x[G][8], big = 0.0f;
@@ -157,8 +159,8 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   const int kr = (r >> 1) + 4 * (r & 1);     // key of a half block that column r stands for
   // the tile's keys that every row of this warp sees, and those that any does
   const int warp_row = row0 + rw * 16, most_row = min(warp_row + 15, run * p.group - 1);
-  const int see_all = len - run + warp_row / p.group + 1;
-  const int see_any = warp_row < run * p.group ? min(len, len - run + most_row / p.group + 1) : 0;
+  const int see_all = len - run + kv4_div(warp_row, p.by_group) + 1;
+  const int see_any = warp_row < run * p.group ? min(len, len - run + kv4_div(most_row, p.by_group) + 1) : 0;
 
   auto consume = [&](auto masked_tag, int tile, int stage, uint32_t there) {
     constexpr bool MASKED = decltype(masked_tag)::value;
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   bool fine = true;
   for (int tile = first; tile < tiles; tile += step) {
     const bool more = rw == 0 && tile + ST * step < tiles;
-    const int64_t ahead = more ? look_up(tile + ST * step) : -1;
+    const uint32_t ahead = more ? look_up(tile + ST * step) : kNoBlock;
     if (!mbar_wait(full + stage * 8, phase)) { fine = false; break; }
     const uint32_t there = held[stage];
     if (tile * 64 < see_any) {
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
         s = fmaf(f, cluster_ld_f32(mapa_u32(whole_at + (w * P4 + 16 * HD + 16 + in) * 4, c)), s);
       }
     }
-    const int at = row0 + row, tok = at / p.group;
+    const int at = row0 + row, tok = kv4_div(at, p.by_group);
     const float inv = s == 0.0f ? 0.0f : 1.0f / s;      // a row that sees nothing is zero
     T* out = static_cast<T*>(p.out) + (q0 + tok) * p.o_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.o_head + d;
     if (p.pair_o) {

@@ -27,7 +27,9 @@ int check_cache(const crl_kv4_cache& c) {
   if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128) return CRL_ERR_SHAPE;
   if (c.page_size <= 0 || c.page_size % kKv4Block != 0 || !aligned16(c.pages)) return CRL_ERR_SHAPE;
   // cache indices are 32-bit, with room for the last tile's end
-  if (static_cast<int64_t>(c.table_width) * c.page_size > INT32_MAX - 1024 || c.num_pages > INT32_MAX) return CRL_ERR_SHAPE;
+  if (static_cast<int64_t>(c.table_width) * c.page_size > INT32_MAX - 1024 || c.num_pages > INT32_MAX ||
+      c.num_pages > (int64_t{0xfffffffe} * kKv4Block) / (static_cast<int64_t>(c.kv_heads) * c.page_size))
+    return CRL_ERR_SHAPE;
   return CRL_OK;
 }
 Kv4Table table_of(const crl_kv4_cache& c) {
@@ -39,7 +41,8 @@ Kv4Table table_of(const crl_kv4_cache& c) {
   t.shift = -1;
   for (int b = 0; b < 30; ++b)
     if (t.blocks == 1 << b) t.shift = b;
-  t.num_pages = c.num_pages;
+  t.num_pages = static_cast<uint32_t>(c.num_pages);
+  t.page_blocks = static_cast<uint32_t>(c.kv_heads) * t.blocks;
   return t;
 }
 bool known16(int dtype) { return dtype == CRL_OUT_F16 || dtype == CRL_OUT_BF16; }
@@ -98,7 +101,7 @@ struct Read {
   }
 };
 
-constexpr int kMaxSplits = 8;      // the portable cluster size
+constexpr int kMaxSplits = 16;      // the largest cluster that the hardware takes (more than 8 are allowed kernel by kernel)
 
 // What is known of an attention kernel on a device: how many clusters of 1 .. kMaxSplits CTAs are resident at once.
 struct KernelFacts {
@@ -110,7 +113,9 @@ int facts_of(K* kernel, KernelFacts* all, int bytes, int threads, KernelFacts** 
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return CRL_ERR_CUDA;
   KernelFacts& f = all[dev];
   if (f.clusters[0].load(std::memory_order_acquire) == 0) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return CRL_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return CRL_ERR_CUDA;
     for (int n = 1; n <= kMaxSplits; ++n) {
       cudaLaunchConfig_t cfg{};
       cfg.gridDim = dim3(n);
@@ -124,7 +129,7 @@ int facts_of(K* kernel, KernelFacts* all, int bytes, int threads, KernelFacts** 
       cfg.numAttrs = 1;
       int many = 0;
       if (cudaOccupancyMaxActiveClusters(&many, kernel, &cfg) != cudaSuccess) return CRL_ERR_CUDA;
-      f.clusters[n].store(many > 0 ? many : 1, std::memory_order_relaxed);
+      f.clusters[n].store(many, std::memory_order_relaxed);      // 0: no GPC has room for as many
     }
     f.clusters[0].store(1, std::memory_order_release);
   }
@@ -140,7 +145,9 @@ int split_keys(const KernelFacts& f, int64_t units, int64_t max_keys, int keys_a
   int64_t least = INT64_MAX;
   for (int n = 1; n <= kMaxSplits; ++n) {
     const int64_t tiles = (max_keys + static_cast<int64_t>(n) * keys_at_once - 1) / (static_cast<int64_t>(n) * keys_at_once);
-    const int64_t active = f.clusters[n].load(std::memory_order_relaxed), waves = (units + active - 1) / active;
+    const int64_t active = f.clusters[n].load(std::memory_order_relaxed);
+    if (active == 0) break;
+    const int64_t waves = (units + active - 1) / active;
     const int64_t cost = waves * (tiles + fixed + (n > 1 ? 1 : 0));
     if (cost < least) {
       least = cost;
@@ -159,10 +166,9 @@ int attend_launch(K* kernel, KernelFacts* all, int bytes, int threads, int tile_
   if (const int rc = facts_of(kernel, all, bytes, threads, &f)) return rc;
   p.row_tiles = (p.max_tokens * p.group + tile_rows - 1) / tile_rows;
   const int64_t units = static_cast<int64_t>(p.seqs) * p.kv_heads * p.row_tiles;
-  if (static_cast<int64_t>(p.kv_heads) * p.row_tiles > 65535) return CRL_ERR_SHAPE;
   const int splits = split_keys(*f, units, max_keys, keys_at_once, 2);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(splits, p.kv_heads * p.row_tiles, p.seqs);
+  cfg.gridDim = dim3(splits * p.row_tiles, p.kv_heads, p.seqs);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
@@ -174,12 +180,19 @@ int attend_launch(K* kernel, KernelFacts* all, int bytes, int threads, int tile_
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const Kv4AttentionParams>(p)) == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
 }
-template <typename T, int HD, int WARPS>
-int attend_few(const Kv4AttentionParams& p, int64_t max_keys, cudaStream_t s) {
-  using Shape = Kv4AttnShape<HD, 1, WARPS>;
+template <typename T, int HD, int COLS, int WARPS>
+int attend_few(Kv4AttentionParams p, int64_t max_keys, cudaStream_t s) {
+  using Shape = Kv4AttnShape<HD, WARPS>;
   static KernelFacts facts[64];
-  return attend_launch(kv4_attention_kernel<T, HD, 1, WARPS>, facts, Shape::kBytes, WARPS * 32, Shape::kRows, WARPS * Shape::kTile * 16, p,
-                       max_keys, s);
+  p.whole_tiles = p.table.blocks % Shape::kTile == 0;
+  return attend_launch(kv4_attention_kernel<T, HD, COLS, WARPS>, facts, Shape::kBytes, WARPS * 32, Shape::kRows, WARPS * Shape::kTile * 16,
+                       p, max_keys, s);
+}
+template <typename T, int HD, int WARPS>
+int attend_few_by_rows(const Kv4AttentionParams& p, int64_t rows, int64_t max_keys, cudaStream_t s) {
+  if (rows * (HD / 32) <= 4) return attend_few<T, HD, 1, WARPS>(p, max_keys, s);
+  if (HD == 32 || rows * (HD / 32) <= 8) return attend_few<T, HD, 2, WARPS>(p, max_keys, s);
+  if constexpr (HD > 32) return attend_few<T, HD, 0, WARPS>(p, max_keys, s);
 }
 template <typename T, int HD, int RW>
 int attend_rows(const Kv4AttentionParams& p, int64_t max_keys, cudaStream_t s) {
@@ -192,10 +205,12 @@ struct Attend {
   static int run(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
     const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group;
     if (rows <= 8) {
-      // few (sequence, key head) pairs need more warps on each than eight CTAs of four
+      // two warps per CTA where there are enough (sequence, key head) pairs to fill the GPU, or so few keys that a CTA of
+      // eight would idle (256 sequences of up to 1024 tokens, 12 heads of 64: 53 us with two, 56 with four, 70 with
+      // eight; 4 sequences of 131k tokens, 8 heads of 128: 270 / 204 / 177 us)
       const int64_t units = static_cast<int64_t>(p.seqs) * p.kv_heads;
-      if (units * kMaxSplits < 4 * sms) return attend_few<T, HD, 8>(p, max_keys, s);
-      return attend_few<T, HD, 4>(p, max_keys, s);
+      if (units >= 2 * sms || max_keys <= 512) return attend_few_by_rows<T, HD, 2>(p, rows, max_keys, s);
+      return attend_few_by_rows<T, HD, 8>(p, rows, max_keys, s);
     }
     if (rows <= 16) return attend_rows<T, HD, 1>(p, max_keys, s);
     if (rows <= 32) return attend_rows<T, HD, 2>(p, max_keys, s);
@@ -268,7 +283,7 @@ int crl_kv4_attention(const crl_kv4_attention_args* a) {
   if (a->q == nullptr || a->out == nullptr || a->lengths == nullptr || a->tokens < 0 || !known16(a->dtype) || a->heads <= 0 ||
       a->max_tokens < 0)
     return CRL_ERR_INVALID;
-  if (a->heads % c.kv_heads != 0 || c.seqs > 65535) return CRL_ERR_SHAPE;
+  if (a->heads % c.kv_heads != 0 || c.seqs > 65535 || c.kv_heads > 65535) return CRL_ERR_SHAPE;
   if (a->tokens == 0 || c.seqs == 0 || a->max_tokens == 0) return CRL_OK;
   int sms = 0;
   if (const int rc = current_sms(&sms)) return rc;
@@ -277,7 +292,10 @@ int crl_kv4_attention(const crl_kv4_attention_args* a) {
   p.table = table_of(c);
   p.lengths = a->lengths; p.cu = a->cu_tokens; p.seqs = c.seqs; p.kv_heads = c.kv_heads; p.group = a->heads / c.kv_heads;
   p.max_tokens = a->cu_tokens != nullptr ? static_cast<int32_t>(std::min<int64_t>(a->max_tokens, a->tokens)) : 1;
-  if (static_cast<int64_t>(p.max_tokens) * p.group > INT32_MAX - 256) return CRL_ERR_SHAPE;
+  const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group + 64;
+  if (rows > (int64_t{1} << 27)) return CRL_ERR_SHAPE;      // leaves the grid room for splits
+  p.by_group.d = static_cast<uint32_t>(p.group);
+  p.by_group.mul = p.group > 1 && rows * p.group < (int64_t{1} << 32) ? static_cast<uint32_t>(((uint64_t{1} << 32) + p.group - 1) / p.group) : 0;
   p.tokens = a->tokens;
   p.q = a->q; p.out = a->out;
   p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.o_tok = a->out_token_stride; p.o_head = a->out_head_stride;
