@@ -47,7 +47,7 @@ struct Kv4AttentionParams {
   void* out;
   int64_t q_tok, q_head, o_tok, o_head;
   int32_t vec_q;
-  int32_t pair_o;             // output rows 4-byte aligned
+  int32_t pair_o, vec_o;      // output rows 4-byte / 16-byte aligned
   int32_t whole_tiles;        // pages hold whole tiles of the kernel
   float scale_log2;           // softmax scale * log2(e)
   int* status;

@@ -8,6 +8,7 @@
 #include "../../include/chessrl_b200.h"
 #include "kv4_append.cuh"
 #include "kv4_attention.cuh"
+#include "kv4_prompt.cuh"
 #include "kv4_rows.cuh"
 #include "logits.cuh"
 
@@ -201,6 +202,22 @@ int attend_rows(const Kv4AttentionParams& p, int64_t max_keys, cudaStream_t s) {
   return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, facts, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, p, max_keys, s);
 }
 template <typename T, int HD>
+int attend_prompt(Kv4AttentionParams p, cudaStream_t s) {
+  using Shape = Kv4PromptShape<HD>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return CRL_ERR_CUDA;
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {      // once per device
+    if (cudaFuncSetAttribute(kv4_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes) != cudaSuccess)
+      return CRL_ERR_CUDA;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  p.row_tiles = (p.max_tokens * p.group + 255) / 256;
+  kv4_prompt_kernel<T, HD><<<dim3(p.row_tiles, p.kv_heads, p.seqs), Shape::kThreads, Shape::kBytes, s>>>(p);
+  return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
+}
+template <typename T, int HD>
 struct Attend {
   static int run(const Kv4AttentionParams& p, int sms, int64_t max_keys, cudaStream_t s) {
     const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group;
@@ -214,6 +231,7 @@ struct Attend {
     }
     if (rows <= 16) return attend_rows<T, HD, 1>(p, max_keys, s);
     if (rows <= 32) return attend_rows<T, HD, 2>(p, max_keys, s);
+    if (rows > 128) return attend_prompt<T, HD>(p, s);
     return attend_rows<T, HD, 4>(p, max_keys, s);
   }
 };
@@ -292,7 +310,7 @@ int crl_kv4_attention(const crl_kv4_attention_args* a) {
   p.table = table_of(c);
   p.lengths = a->lengths; p.cu = a->cu_tokens; p.seqs = c.seqs; p.kv_heads = c.kv_heads; p.group = a->heads / c.kv_heads;
   p.max_tokens = a->cu_tokens != nullptr ? static_cast<int32_t>(std::min<int64_t>(a->max_tokens, a->tokens)) : 1;
-  const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group + 64;
+  const int64_t rows = static_cast<int64_t>(p.max_tokens) * p.group + 256;      // a tile's last row
   if (rows > (int64_t{1} << 27)) return CRL_ERR_SHAPE;      // leaves the grid room for splits
   p.by_group.d = static_cast<uint32_t>(p.group);
   p.by_group.mul = p.group > 1 && rows * p.group < (int64_t{1} << 32) ? static_cast<uint32_t>(((uint64_t{1} << 32) + p.group - 1) / p.group) : 0;
@@ -301,6 +319,7 @@ int crl_kv4_attention(const crl_kv4_attention_args* a) {
   p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.o_tok = a->out_token_stride; p.o_head = a->out_head_stride;
   p.vec_q = rows_aligned(a->q, p.q_tok, p.q_head);
   p.pair_o = (reinterpret_cast<uintptr_t>(a->out) & 3) == 0 && p.o_tok % 2 == 0 && p.o_head % 2 == 0;
+  p.vec_o = rows_aligned(a->out, p.o_tok, p.o_head);
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.status = a->device_status;
   return by_type<Attend>(a->dtype, c.head_dim, p, sms, static_cast<int64_t>(c.table_width) * c.page_size,

@@ -228,6 +228,9 @@ def test_attention_over_page_sizes_and_splits(crl, page):
     (F16, 64, 6, 2, [(70, 210), (0, 5), (128, 128)]),
     (BF16, 32, 8, 8, [(200, 333)]),
     (F16, 128, 8, 2, [(150, 150), (65, 1100)]),
+    (F16, 128, 4, 1, [(700, 1500), (1, 1), (300, 333)]),
+    (BF16, 64, 3, 1, [(900, 901), (0, 70), (257, 600)]),
+    (F16, 32, 4, 2, [(500, 640), (129, 129)]),
 ])
 def test_attention_of_runs_and_prompts(crl, dtype, hd, heads, kv, runs):
     attend_case(crl, dtype, hd, heads, kv, 32, runs, seed=hd + heads + len(runs))
@@ -236,7 +239,7 @@ def test_attention_of_runs_and_prompts(crl, dtype, hd, heads, kv, runs):
 def test_rows_that_see_nothing_are_zero(crl):
     """A run longer than what the cache holds: its first rows stand before the first key."""
     gen = torch.Generator().manual_seed(2)
-    for n, length in ((4, 2), (40, 10), (3, 0)):
+    for n, length in ((4, 2), (40, 10), (3, 0), (400, 150)):
         pages, table = filled(crl, [max(length, 1)], 16, 2, 64, gen)
         q = torch.randn(n, 4, 64, generator=gen).half().cuda()
         out = crl.kv4_attention(pages, q, table, ints([length]), cu_tokens=ints([0, n]), max_tokens=n)
@@ -253,12 +256,16 @@ def test_attention_of_extreme_scales(crl, dtype):
     attend_case(crl, dtype, 32, 4, 2, 16, [(1, 200), (1, 3)], seed=3, key_scale=30.0)
     attend_case(crl, dtype, 128, 4, 2, 16, [(1, 200), (40, 63)], seed=4, scale=0.0)
     attend_case(crl, dtype, 64, 4, 2, 16, [(2, 200), (1, 1)], seed=5, scale=-0.3)
+    attend_case(crl, dtype, 64, 4, 2, 16, [(200, 400)], seed=6, value_scale=1e-4)
+    attend_case(crl, dtype, 128, 4, 2, 16, [(200, 300)], seed=7, q_scale=1e-3, scale=-0.2)
+    attend_case(crl, dtype, 32, 4, 2, 16, [(200, 300)], seed=8, key_scale=30.0)
+    attend_case(crl, dtype, 64, 4, 2, 16, [(150, 300)], seed=9, scale=0.0)
 
 
 def test_values_growing_along_the_sequence(crl):
     """The running exponent of the values' steps has to rise tile after tile."""
     gen = torch.Generator().manual_seed(9)
-    for n in (1, 40):
+    for n in (1, 40, 300):
         pages, table = pool(crl, [700], 64, 1, 64, gen)
         k = torch.randn(700, 1, 64, generator=gen).half().cuda()
         v = (torch.randn(700, 1, 64, generator=gen) * torch.linspace(-7, 9, 700).exp2()[:, None, None]).half().cuda()
@@ -268,23 +275,38 @@ def test_values_growing_along_the_sequence(crl):
         check_attention(out, q, pages, table, [(n, 700)])
 
 
-@pytest.mark.parametrize("n", [1, 4, 40])
+@pytest.mark.parametrize("n", [1, 4, 40, 150])
 def test_hidden_rows_do_not_leak(crl, n):
     """NaN in later tokens of the run and in the rest of the page (the pool is filled with NaN steps) stays out of the rows
     that do not see it; in what a row does see it shows."""
     gen = torch.Generator().manual_seed(4)
-    pages, table = pool(crl, [50], 32, 2, 64, gen)
-    k = torch.randn(50, 2, 64, generator=gen).half()
-    k[49, 0] = math.nan
-    v = torch.randn(50, 2, 64, generator=gen).half()
-    v[49, 0, 40] = math.nan
-    crl.kv4_append(pages, k.cuda(), v.cuda(), table, ints([0]), cu_tokens=ints([0, 50]))
+    held = max(50, n + 9)
+    pages, table = pool(crl, [held], 32, 2, 64, gen)
+    k = torch.randn(held, 2, 64, generator=gen).half()
+    k[held - 1, 0] = math.nan
+    v = torch.randn(held, 2, 64, generator=gen).half()
+    v[held - 1, 0, 40] = math.nan
+    crl.kv4_append(pages, k.cuda(), v.cuda(), table, ints([0]), cu_tokens=ints([0, held]))
     q = torch.randn(n, 2, 64, generator=gen).half().cuda()
-    out = crl.kv4_attention(pages, q, table, ints([50]), cu_tokens=ints([0, n]), max_tokens=n)
+    out = crl.kv4_attention(pages, q, table, ints([held]), cu_tokens=ints([0, n]), max_tokens=n)
     assert torch.isfinite(out[:n - 1]).all() and torch.isfinite(out[:, 1]).all()
     assert torch.isnan(out[n - 1, 0]).all()
-    out = crl.kv4_attention(pages, q, table, ints([49]), cu_tokens=ints([0, n]), max_tokens=n)
-    check_attention(out, q, pages, table, [(n, 49)])
+    out = crl.kv4_attention(pages, q, table, ints([held - 1]), cu_tokens=ints([0, n]), max_tokens=n)
+    check_attention(out, q, pages, table, [(n, held - 1)])
+
+
+@pytest.mark.parametrize("n", [2, 40, 150])
+def test_a_nan_value_reaches_its_group_of_the_rows_that_see_it(crl, n):
+    gen = torch.Generator().manual_seed(8)
+    held, hit = n + 20, 20 + n // 2
+    pages, table = pool(crl, [held], 16, 1, 64, gen)
+    k, v = torch.randn(held, 1, 64, generator=gen).half(), torch.randn(held, 1, 64, generator=gen).half()
+    v[hit, 0, 40] = math.nan
+    crl.kv4_append(pages, k.cuda(), v.cuda(), table, ints([0]), cu_tokens=ints([0, held]))
+    q = torch.randn(n, 2, 64, generator=gen).half().cuda()
+    out = crl.kv4_attention(pages, q, table, ints([held]), cu_tokens=ints([0, n]), max_tokens=n)
+    sees = hit - 20      # the first row that does
+    assert torch.isfinite(out[:sees]).all() and torch.isfinite(out[:, :, :32]).all() and torch.isnan(out[sees:, :, 32:]).all()
 
 
 def test_attention_with_strides_and_padding(crl):
