@@ -3,8 +3,10 @@
 // Same contract as kv4_attention_kernel. A CTA takes 256 query rows of a (sequence, key head) as two tiles of 128 and walks
 // the keys in tiles of KT. Its warps:
 //   0-3, 4-7   softmax of the first / second row tile: a thread owns a row
-//   8-15       unpack: warp 8 + b turns block b of a key tile into matrix operands in shared memory
-//   16         one thread issues the tcgen05.mma products; the warp owns the tensor memory
+//   8-14       unpack: warp 8 + b turns block b of a key tile into matrix operands in shared memory
+//   15         one thread issues the tcgen05.mma products; the warp owns the tensor memory
+// The softmax warps take registers over from the others (168 and 88 of the 128 at launch), so that a row's 112 scores are
+// read from tensor memory once and stay in registers.
 // Tensor memory: scores S [128 x KT] fp32 per row tile, over which the weights P are written back as f16 (the left
 // operand of the output product), and the outputs O [128 x (hd + 16)] fp32: 512 columns in all at hd 128, KT 112.
 // The two row tiles are half a step apart: while one's softmax runs, the other's products do.
@@ -28,7 +30,7 @@ namespace crl {
 
 template <int HD>
 struct Kv4PromptShape {
-  static constexpr int kKeys = HD == 128 ? 112 : 128;     // the most that S and O leave room for in tensor memory
+  static constexpr int kKeys = 112;      // the most that S and O leave room for in tensor memory at hd 128
   static constexpr int kBlocks = kKeys / 16;
   static constexpr int kWide = HD + 16;                   // dims and the centres' columns
   static constexpr int kLeadQ = 128 * 16, kLeadK = kKeys * 16 + 32, kLeadV = kWide * 16;
@@ -38,7 +40,7 @@ struct Kv4PromptShape {
   static constexpr int kOffBad = kOffFlags + 4 * 8 * 4;            // 4 x kKeys bytes: groups of a key's value that are NaN
   static constexpr int kOffBars = (kOffBad + 4 * kKeys + 15) / 16 * 16;
   static constexpr int kBytes = kOffBars + 16 * 8;
-  static constexpr int kThreads = 17 * 32;
+  static constexpr int kThreads = 16 * 32;
   static constexpr int kColS = 0, kColO = 2 * kKeys;      // tensor memory columns: S_a, S_b, O_a, O_b
 };
 
@@ -76,6 +78,28 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t addr, const uint32_t (&r)[8]
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_kernel(const Kv4AttentionParams p) {
@@ -124,7 +148,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     }
     mbar_fence_init();
   }
-  if (warp == 16) {
+  if (warp == 15) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -190,8 +214,10 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool fine = true;
-
-  if (warp == 16) {
+  if (warp >= 8) {
+    // registers: 256 x 168 + 256 x 88 = 512 x 128
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 15) {
     // ---- products ---------------------------------------------------------------------------------------------------
     if (lane == 0 && tiles > 0) {
       const uint32_t idesc_s = umma_idesc(128, KT, 0, 1), idesc_o = umma_idesc(128, Shape::kWide, 0, 1);
@@ -238,10 +264,10 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       for (int x = 0; x < 2; ++x) fine = mbar_wait(o_done + 8 * x, (tiles - 1) & 1) && fine;
     }
     __syncwarp();
-  } else if (warp >= 8) {
+    } else {
     // ---- unpack -----------------------------------------------------------------------------------------------------
     const int b = warp - 8;
-    if (b < NB) {
+    {
       const int32_t* pages_of = p.table.table + seq * p.table.stride;
       const uint8_t* head_pages = p.pages + static_cast<size_t>(head) * p.table.blocks * BB;
       const int kt = lane & 3, kn = lane >> 2;                 // keys kn, kn + 8, quarter kt
@@ -286,15 +312,18 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
           lds_words<VG>(vm[j], from + 18 * HD + (8 * vc + j) * (G * 4) + vg * 4);
         }
       };
+      // the table is read two tiles ahead, the codes one
       from = tiles > 0 ? look(0) : nullptr;
       if (tiles > 0) {
         load_keys();
         load_values();
       }
+      bool there = from != nullptr;
+      const uint8_t* then = tiles > 1 ? look(1) : nullptr;
       for (int i = 0; i < tiles; ++i) {
         const int stage = i & 1;
-        const bool there = from != nullptr;
-        from = i + 1 < tiles ? look(i + 1) : nullptr;
+        from = then;
+        then = i + 2 < tiles ? look(i + 2) : nullptr;
         if (i >= 2 && !mbar_wait(k_free + 8 * stage, ((i >> 1) & 1) ^ 1)) { fine = false; break; }
         uint8_t* k = smem + Shape::kOffK + stage * Shape::kK;
 #pragma unroll
@@ -385,10 +414,13 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_full + 8 * stage);
+        there = from != nullptr;
       }
+    }
     }
   } else {
     // ---- softmax: thread = row --------------------------------------------------------------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int x = warp >> 2, row = threadIdx.x & 127, mine = x * 128 + row, at = row0 + mine;
     const int tok = kv4_div(at, p.by_group);
     const bool on = mine < live;
@@ -410,23 +442,24 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
           if (((broken >> (k >> 4)) & 1u) && i * KT + k < limit) lost |= bad_keys[(i & 3) * KT + k];
         __syncwarp();
       }
-      auto hide = [&](uint32_t (&v)[16], int c) {      // 16 columns = one block
-        const int first = i * KT + 16 * c;
-        const bool gone = !((there >> c) & 1u);
+      uint32_t v[NB][16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (gone || first + j >= limit) v[j] = 0xff800000u;
-      };
+      for (int c = 0; c < NB; ++c) tmem_ld_x16(s_at + 16 * c, v[c]);
+      tmem_ld_wait();
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {      // 16 columns = one block
+          const int first = ((there >> c) & 1u) ? i * KT + 16 * c : INT32_MAX - 16;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (first + j >= limit) v[c][j] = 0xff800000u;
+        }
+      }
       float most = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < NB; ++c) {
-        uint32_t v[16];
-        tmem_ld_x16(s_at + 16 * c, v);
-        tmem_ld_wait();
-        if (masked) hide(v, c);
+      for (int c = 0; c < NB; ++c)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) most = fmaxf(most, __uint_as_float(v[j]));
-      }
+        for (int j = 0; j < 16; j += 2) most = max3(most, __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
       const float next = most == -INFINITY ? -INFINITY : most * factor;
       if (i == 0) {
         top = next;
@@ -437,34 +470,39 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
         sum *= alpha;
 #pragma unroll 1
         for (int c = 0; c < Shape::kWide; c += 16) {
-          uint32_t v[16];
-          tmem_ld_x16(o_at + c, v);
+          uint32_t o[16];
+          tmem_ld_x16(o_at + c, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-          tmem_st_x16(o_at + c, v);
+          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+          tmem_st_x16(o_at + c, o);
         }
       }
       const float off = top == -INFINITY ? 0.0f : top;
+      const uint64_t factor2 = pack_f32x2(factor, factor), off2 = pack_f32x2(-off, -off);
+      uint64_t sum2 = 0;
 #pragma unroll
       for (int c = 0; c < NB; ++c) {
-        uint32_t v[16], w[8];
-        tmem_ld_x16(s_at + 16 * c, v);
-        tmem_ld_wait();
-        if (masked) hide(v, c);
+        uint32_t w[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float raw = __uint_as_float(v[j]);
-          float e = fmaf(raw, factor, -off);
-          if (masked && raw == -INFINITY) e = -INFINITY;      // also where the factor is zero
-          e = exp2_approx(e);
-          sum += e;
-          v[j] = __float_as_uint(e);
+        for (int j = 0; j < 16; j += 2) {
+          const float r0 = __uint_as_float(v[c][j]), r1 = __uint_as_float(v[c][j + 1]);
+          float e0, e1;
+          unpack_f32x2(fma_f32x2(pack_f32x2(r0, r1), factor2, off2), e0, e1);
+          if (masked) {      // also where the factor is zero
+            if (r0 == -INFINITY) e0 = -INFINITY;
+            if (r1 == -INFINITY) e1 = -INFINITY;
+          }
+          e0 = exp2_approx(e0);
+          e1 = exp2_approx(e1);
+          sum2 = add_f32x2(sum2, pack_f32x2(e0, e1));
+          w[j / 2] = pack_f16(e0, e1);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = pack_f16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
         tmem_st_x8(s_at + 8 * c, w);
       }
+      float sum_a, sum_b;
+      unpack_f32x2(sum2, sum_a, sum_b);
+      sum += sum_a + sum_b;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -507,7 +545,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
   if (!fine && lane == 0) kv4_report(p.status, kDevKv4Timeout);
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 15) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
