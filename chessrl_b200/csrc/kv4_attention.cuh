@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) kv4_attention_kernel(c
       sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
       sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
     }
-    const float factor = __uint_as_float(static_cast<uint32_t>(127 + 24 + e) << 23) * fabsf(p.scale_log2);
+    // never zero, so that a hidden score stays at minus infinity
+    const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + 24 + e) << 23) * fabsf(p.scale_log2), 1e-35f);
     const int lim = on ? len - run + tok + 1 : 0;
     // lane (r, t) needs columns 2t and 2t + 1: lanes 4 * (2t) and 4 * (2t + 1) hold them
 #pragma unroll
@@ -339,8 +340,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) kv4_attention_kernel(c
     for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int m = 4; m < 32; m <<= 1) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], m));
-      // the maximum in log2 units, less 3; a hidden row's stays at minus infinity whatever its factor
-      most[c] = fmaxf(top[c], most[c] == -INFINITY ? -INFINITY : fmaf(most[c], kcol[c], -3.0f));
+      most[c] = fmaxf(top[c], fmaf(most[c], kcol[c], -3.0f));      // the maximum in log2 units, less 3
     }
     if (__any_sync(0xffffffffu, most[0] > top[0] || (C == 2 && most[1] > top[1]))) {
       float alpha[2];
@@ -367,9 +367,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) kv4_attention_kernel(c
     for (int b = 0; b < TB; ++b)
 #pragma unroll
       for (int i = 0; i < 4; i += 3 - C) {
-        float x = fmaf(sc[b][i], kcol[i & 1], -off[i & 1]);
-        if (MASKED && sc[b][i] == -INFINITY) x = -INFINITY;      // also where the factor is zero
-        sc[b][i] = exp2_approx(x);
+        sc[b][i] = exp2_approx(fmaf(sc[b][i], kcol[i & 1], -off[i & 1]));
         sum[i & 1] += sc[b][i];
       }
     // output

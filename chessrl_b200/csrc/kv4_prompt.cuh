@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       if (part == 0) {
         *reinterpret_cast<uint4*>(q + HD / 8 * Shape::kLeadQ) = make_uint4(lead[0], lead[1], rest[0], rest[1]);
         *reinterpret_cast<uint4*>(q + (HD / 8 + 1) * Shape::kLeadQ) = make_uint4(0, 0, 0, 0);
-        factors[row] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(p.scale_log2);
+        // never zero, so that a hidden score stays at minus infinity
+        factors[row] = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(p.scale_log2), 1e-35f);
       }
     }
   }
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       for (int c = 0; c < NB; ++c)
 #pragma unroll
         for (int j = 0; j < 16; j += 2) most = max3(most, __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
-      const float next = most == -INFINITY ? -INFINITY : most * factor;
+      const float next = most * factor;
       if (i == 0) {
         top = next;
       } else if (__any_sync(0xffffffffu, next > top + 8.0f || (top == -INFINITY && next > top))) {
@@ -489,10 +490,6 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
           const float r0 = __uint_as_float(v[c][j]), r1 = __uint_as_float(v[c][j + 1]);
           float e0, e1;
           unpack_f32x2(fma_f32x2(pack_f32x2(r0, r1), factor2, off2), e0, e1);
-          if (masked) {      // also where the factor is zero
-            if (r0 == -INFINITY) e0 = -INFINITY;
-            if (r1 == -INFINITY) e1 = -INFINITY;
-          }
           e0 = exp2_approx(e0);
           e1 = exp2_approx(e1);
           sum2 = add_f32x2(sum2, pack_f32x2(e0, e1));
