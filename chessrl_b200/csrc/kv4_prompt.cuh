@@ -346,27 +346,31 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
         load_keys();
         // a value row that no query sees may hold anything; one that is NaN must not reach the rows that do not see it
         // through 0 * NaN: it is taken out here and given to the rows that see it by the softmax warps
-        uint32_t bad[8], any = 0;
+        if (!there || i * KT + b * 16 + 16 > seen_most) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          bad[j] = 0;
-          const bool gone = !there || i * KT + b * 16 + 8 * vc + j >= seen_most;
+          for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int g = 0; g < VG; ++g) {
-            if (gone) vm[j][g] = 0;
-            if ((vm[j][g] & 0x7c00u) == 0x7c00u || (vm[j][g] & 0x7c000000u) == 0x7c000000u) {
-              bad[j] |= 1u << (vg + g);
-              vm[j][g] = 0;
-            }
-          }
-          any |= bad[j];
+            for (int g = 0; g < VG; ++g)
+              if (!there || i * KT + b * 16 + 8 * vc + j >= seen_most) vm[j][g] = 0;
         }
-        const bool some = __any_sync(0xffffffffu, any != 0);
+        __half2 probe = __float2half2_rn(0.0f);      // 0 * m is NaN for a NaN or an infinity
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int g = 0; g < VG; ++g) probe = __hfma2(as_half2(vm[j][g]), __float2half2_rn(0.0f), probe);
+        const bool some = __any_sync(0xffffffffu, (as_word(probe) & 0x7fff7fffu) != 0);
         if (some) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            bad[j] |= __shfl_xor_sync(0xffffffffu, bad[j], 8);      // the other half's groups
-            if (vr == 0 && vh == 0) bad_keys[(i & 3) * KT + b * 16 + 8 * vc + j] = static_cast<uint8_t>(bad[j]);
+            uint32_t bad = 0;
+#pragma unroll
+            for (int g = 0; g < VG; ++g)
+              if ((vm[j][g] & 0x7c00u) == 0x7c00u || (vm[j][g] & 0x7c000000u) == 0x7c000000u) {
+                bad |= 1u << (vg + g);
+                vm[j][g] = 0;
+              }
+            bad |= __shfl_xor_sync(0xffffffffu, bad, 8);      // the other half's groups
+            if (vr == 0 && vh == 0) bad_keys[(i & 3) * KT + b * 16 + 8 * vc + j] = static_cast<uint8_t>(bad);
           }
         }
         if (lane == 0) flags[(i & 3) * 8 + b] = (there ? 1u : 0u) | (some ? 2u : 0u);
