@@ -39,7 +39,7 @@ struct Kv4PromptShape {
   static constexpr int kOffFlags = kOffRows + 256 * 4;             // the rows' factors, then 4 x 8 words of block flags
   static constexpr int kOffBad = kOffFlags + 4 * 8 * 4;            // 4 x kKeys bytes: groups of a key's value that are NaN
   static constexpr int kOffBars = (kOffBad + 4 * kKeys + 15) / 16 * 16;
-  static constexpr int kBytes = kOffBars + 16 * 8;
+  static constexpr int kBytes = kOffBars + 18 * 8;
   static constexpr int kThreads = 16 * 32;
   static constexpr int kColS = 0, kColO = 2 * kKeys;      // tensor memory columns: S_a, S_b, O_a, O_b
 };
@@ -95,16 +95,12 @@ __device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_kernel(const Kv4AttentionParams p) {
   using Shape = Kv4PromptShape<HD>;
   constexpr int G = HD / 32, BB = kv4_block_bytes(HD), KT = Shape::kKeys, NB = Shape::kBlocks;
+  constexpr int kHalf = 4;      // blocks of a tile whose weights are handed over early
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.y, row_tile = p.row_tiles - 1 - static_cast<int>(blockIdx.x), seq = blockIdx.z;   // long rows first
@@ -133,8 +129,8 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
   const uint32_t bars = smem_u32(smem + Shape::kOffBars);
   // full / free per operand stage, then per row tile: scores there, weights there, output product done
   const uint32_t k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, p_full = bars + 80,
-                 o_done = bars + 96;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Shape::kOffBars + 112);
+                 o_done = bars + 96, p_half = bars + 112;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Shape::kOffBars + 128);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
@@ -143,6 +139,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       mbar_init(v_full + 8 * s, NB);
       mbar_init(v_free + 8 * s, 1);
       mbar_init(s_full + 8 * s, 2);      // the products' commit and the issuing thread
+      mbar_init(p_half + 8 * s, 4);
       mbar_init(p_full + 8 * s, 4);
       mbar_init(o_done + 8 * s, 1);
     }
@@ -152,14 +149,17 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
-  // the centres' columns that no group has stay zero: clear both stages' extra columns
+  // both stages' extra columns: those that no group has are zero for good, one of the values' is one: it collects the
+  // rows' sums of P
+  constexpr int kSumRow = 4;
   for (int i = threadIdx.x; i < 2 * 2 * KT; i += Shape::kThreads) {
     const int stage = i / (2 * KT), c = i / KT % 2, row = i % KT;
     *reinterpret_cast<uint4*>(smem + Shape::kOffK + stage * Shape::kK + (HD / 8 + c) * Shape::kLeadK + row * 16) = make_uint4(0, 0, 0, 0);
   }
   for (int i = threadIdx.x; i < 2 * (KT / 8) * 16; i += Shape::kThreads) {
     const int stage = i / (KT / 8 * 16), c = i / 16 % (KT / 8), row = i % 16;
-    *reinterpret_cast<uint4*>(smem + Shape::kOffV + stage * Shape::kV + c * Shape::kLeadV + (HD + row) * 16) = make_uint4(0, 0, 0, 0);
+    const uint32_t one = row == kSumRow ? 0x3c003c00u : 0u;
+    *reinterpret_cast<uint4*>(smem + Shape::kOffV + stage * Shape::kV + c * Shape::kLeadV + (HD + row) * 16) = make_uint4(one, one, one, one);
   }
   // queries: HD / 8 lanes a row
   {
@@ -242,14 +242,20 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       for (int i = 0; i < tiles && fine; ++i) {
 #pragma unroll 1
         for (int x = 0; x < 2 && fine; ++x) {
-          fine = mbar_wait(p_full + 8 * x, i & 1) && (x == 1 || mbar_wait(v_full + 8 * (i & 1), (i >> 1) & 1));
+          fine = mbar_wait(p_half + 8 * x, i & 1) && (x == 1 || mbar_wait(v_full + 8 * (i & 1), (i >> 1) & 1));
           if (!fine) break;
           tc_fence_after();
           const uint32_t v = sm + Shape::kOffV + (i & 1) * Shape::kV, o = tmem + Shape::kColO + x * Shape::kWide;
 #pragma unroll
-          for (int s = 0; s < KT / 16; ++s)
+          for (int s = 0; s < kHalf; ++s)
             umma_f16_ta(o, tmem + Shape::kColS + x * KT + 8 * s, umma_desc_plain(v + 2 * s * Shape::kLeadV, Shape::kLeadV), idesc_o,
                         i > 0 || s > 0);
+          fine = mbar_wait(p_full + 8 * x, i & 1);
+          if (!fine) break;
+          tc_fence_after();
+#pragma unroll
+          for (int s = kHalf; s < KT / 16; ++s)
+            umma_f16_ta(o, tmem + Shape::kColS + x * KT + 8 * s, umma_desc_plain(v + 2 * s * Shape::kLeadV, Shape::kLeadV), idesc_o, 1);
           tc_commit(o_done + 8 * x);
           if (x == 1) tc_commit(v_free + 8 * (i & 1));
           if (i + 1 < tiles) {
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     const float factor = factors[mine];
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;      // 32 tensor memory lanes a warp
     const uint32_t s_at = tmem + lanes + Shape::kColS + x * KT, o_at = tmem + lanes + Shape::kColO + x * Shape::kWide;
-    float top = -INFINITY, sum = 0.0f;      // maximum in use, log2 units
+    float top = -INFINITY;                  // maximum in use, log2 units
     uint32_t lost = 0;                      // groups that a NaN value has reached
     for (int i = 0; i < tiles; ++i) {
       if (!mbar_wait(s_full + 8 * x, i & 1)) { fine = false; break; }
@@ -460,11 +466,12 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
             if (first + j >= limit) v[c][j] = 0xff800000u;
         }
       }
-      float most = -INFINITY;
+      float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < NB; ++c)
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) most = max3(most, __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
+        for (int j = 0; j < 16; j += 2) high[j / 2 % 4] = max3(high[j / 2 % 4], __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
+      const float most = fmaxf(max3(high[0], high[1], high[2]), high[3]);
       const float next = most * factor;
       if (i == 0) {
         top = next;
@@ -472,7 +479,6 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
         // the output product of the step before is through (the scores were issued after it)
         const float now = fmaxf(top, next), alpha = top == -INFINITY ? 0.0f : exp2_approx(top - now);
         top = now;
-        sum *= alpha;
 #pragma unroll 1
         for (int c = 0; c < Shape::kWide; c += 16) {
           uint32_t o[16];
@@ -485,25 +491,23 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       }
       const float off = top == -INFINITY ? 0.0f : top;
       const uint64_t factor2 = pack_f32x2(factor, factor), off2 = pack_f32x2(-off, -off);
-      uint64_t sum2 = 0;
 #pragma unroll
       for (int c = 0; c < NB; ++c) {
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          const float r0 = __uint_as_float(v[c][j]), r1 = __uint_as_float(v[c][j + 1]);
           float e0, e1;
-          unpack_f32x2(fma_f32x2(pack_f32x2(r0, r1), factor2, off2), e0, e1);
-          e0 = exp2_approx(e0);
-          e1 = exp2_approx(e1);
-          sum2 = add_f32x2(sum2, pack_f32x2(e0, e1));
-          w[j / 2] = pack_f16(e0, e1);
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])), factor2, off2), e0, e1);
+          w[j / 2] = pack_f16(exp2_approx(e0), exp2_approx(e1));
         }
         tmem_st_x8(s_at + 8 * c, w);
+        if (c == kHalf - 1) {      // the output product can start on these
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_half + 8 * x);
+        }
       }
-      float sum_a, sum_b;
-      unpack_f32x2(sum2, sum_a, sum_b);
-      sum += sum_a + sum_b;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -513,13 +517,13 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       fine = mbar_wait(o_done + 8 * x, (tiles - 1) & 1);
       tc_fence_after();
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;      // a row that sees nothing is zero
     T* out = static_cast<T*>(p.out) + (q0 + tok) * p.o_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.o_head;
     uint32_t cen[16];
     if (fine && tiles > 0) {
       tmem_ld_x16(o_at + HD, cen);
       tmem_ld_wait();
     }
+    const float sum = tiles > 0 ? __uint_as_float(cen[kSumRow]) : 0.0f, inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // 0: sees nothing
 #pragma unroll
     for (int c = 0; c < HD; c += 16) {
       uint32_t v[16];
