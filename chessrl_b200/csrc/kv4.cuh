@@ -86,16 +86,23 @@ template <typename T> __device__ __forceinline__ T kv4_from_float(float x);
 template <> __device__ __forceinline__ __half kv4_from_float(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 kv4_from_float(float x) { return __float2bfloat16_rn(x); }
 
-// eight consecutive values; `vec`: 16-byte aligned
+// eight consecutive values as they are; `vec`: 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void kv4_load8(const T* p, bool vec, float (&x)[8]) {
-  T t[8];
-  if (vec) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
-  else
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = p[i];
+__device__ __forceinline__ uint4 kv4_raw8(const T* p, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(p);
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  return make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16, h[4] | static_cast<uint32_t>(h[5]) << 16,
+                    h[6] | static_cast<uint32_t>(h[7]) << 16);
+}
+template <typename T>
+__device__ __forceinline__ void kv4_floats8(const uint4& raw, float (&x)[8]) {
+  const T* t = reinterpret_cast<const T*>(&raw);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = kv4_to_float(t[i]);
+}
+template <typename T>
+__device__ __forceinline__ void kv4_load8(const T* p, bool vec, float (&x)[8]) {
+  kv4_floats8<T>(kv4_raw8(p, vec), x);
 }
 template <typename T>
 __device__ __forceinline__ void kv4_store8(T* p, bool vec, const float (&x)[8]) {

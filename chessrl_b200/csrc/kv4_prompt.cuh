@@ -35,11 +35,11 @@ struct Kv4PromptShape {
   static constexpr int kWide = HD + 16;                   // dims and the centres' columns
   static constexpr int kLeadQ = 128 * 16, kLeadK = kKeys * 16 + 32, kLeadV = kWide * 16;
   static constexpr int kQ = kWide / 8 * kLeadQ, kK = kWide / 8 * kLeadK, kV = kKeys / 8 * kLeadV;
-  static constexpr int kOffK = 2 * kQ, kOffV = kOffK + 2 * kK, kOffRows = kOffV + 2 * kV;
-  static constexpr int kOffFlags = kOffRows + 256 * 4;             // the rows' factors, then 4 x 8 words of block flags
+  static constexpr int kOffK = 2 * kQ, kOffV = kOffK + 2 * kK;
+  static constexpr int kOffFlags = kOffV + 2 * kV;                 // 4 x 8 words of block flags
   static constexpr int kOffBad = kOffFlags + 4 * 8 * 4;            // 4 x kKeys bytes: groups of a key's value that are NaN
   static constexpr int kOffBars = (kOffBad + 4 * kKeys + 15) / 16 * 16;
-  static constexpr int kBytes = kOffBars + 18 * 8;
+  static constexpr int kBytes = kOffBars + 20 * 8;
   static constexpr int kThreads = 16 * 32;
   static constexpr int kColS = 0, kColO = 2 * kKeys;      // tensor memory columns: S_a, S_b, O_a, O_b
 };
@@ -123,14 +123,13 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
   const int seen_most = max(0, min(len, len - run + last_tok + 1));
   const int tiles = (seen_most + KT - 1) / KT;
 
-  float* factors = reinterpret_cast<float*>(smem + Shape::kOffRows);
   uint32_t* flags = reinterpret_cast<uint32_t*>(smem + Shape::kOffFlags);
   uint8_t* bad_keys = smem + Shape::kOffBad;
   const uint32_t bars = smem_u32(smem + Shape::kOffBars);
   // full / free per operand stage, then per row tile: scores there, weights there, output product done
   const uint32_t k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, p_full = bars + 80,
-                 o_done = bars + 96, p_half = bars + 112;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Shape::kOffBars + 128);
+                 o_done = bars + 96, p_half = bars + 112, q_full = bars + 128;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Shape::kOffBars + 144);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
@@ -138,6 +137,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       mbar_init(k_free + 8 * s, 1);
       mbar_init(v_full + 8 * s, NB);
       mbar_init(v_free + 8 * s, 1);
+      mbar_init(q_full + 8 * s, 4);
       mbar_init(s_full + 8 * s, 2);      // the products' commit and the issuing thread
       mbar_init(p_half + 8 * s, 4);
       mbar_init(p_full + 8 * s, 4);
@@ -160,54 +160,6 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     const int stage = i / (KT / 8 * 16), c = i / 16 % (KT / 8), row = i % 16;
     const uint32_t one = row == kSumRow ? 0x3c003c00u : 0u;
     *reinterpret_cast<uint4*>(smem + Shape::kOffV + stage * Shape::kV + c * Shape::kLeadV + (HD + row) * 16) = make_uint4(one, one, one, one);
-  }
-  // queries: HD / 8 lanes a row
-  {
-    constexpr int LANES = HD / 8, AT_ONCE = Shape::kThreads / LANES;
-    const int part = lane % LANES;
-    for (int base = 0; base < 256; base += AT_ONCE) {
-      const int row = base + threadIdx.x / LANES;
-      const bool there = row < 256;
-      const int at = row0 + row, tok = kv4_div(at, p.by_group);
-      const bool on = there && row < live;
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, big = 0.0f, sum = 0.0f;
-      if (on)
-        kv4_load8(static_cast<const T*>(p.q) + (q0 + tok) * p.q_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.q_head + part * 8,
-                  p.vec_q, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));
-#pragma unroll
-      for (int m = 1; m < LANES; m <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
-      const int e = big > 0.0f ? min(120, max(-120, static_cast<int>(__float_as_uint(big) >> 23) - 127)) : 0;
-      // a negative scale is taken into q, so that the largest score is the largest product
-      const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.scale_log2);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] *= down;
-        sum += x[i];
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const __half hi = __float2half_rn(sum);
-      const uint32_t both = as_word(__halves2half2(hi, __float2half_rn(sum - __half2float(hi))));
-      uint32_t lead[2] = {0, 0}, rest[2] = {0, 0};
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint32_t b = __shfl_sync(0xffffffffu, both, (lane - part) + 4 * g);
-        lead[g / 2] |= (b & 0xffffu) << (16 * (g & 1));
-        rest[g / 2] |= (b >> 16) << (16 * (g & 1));
-      }
-      if (!there) continue;
-      uint8_t* q = smem + (row >> 7) * Shape::kQ + ((row & 127) >> 3) * 128 + (row & 7) * 16;
-      *reinterpret_cast<uint4*>(q + part * Shape::kLeadQ) =
-          make_uint4(pack_f16(x[0], x[4]), pack_f16(x[1], x[5]), pack_f16(x[2], x[6]), pack_f16(x[3], x[7]));
-      if (part == 0) {
-        *reinterpret_cast<uint4*>(q + HD / 8 * Shape::kLeadQ) = make_uint4(lead[0], lead[1], rest[0], rest[1]);
-        *reinterpret_cast<uint4*>(q + (HD / 8 + 1) * Shape::kLeadQ) = make_uint4(0, 0, 0, 0);
-        // never zero, so that a hidden score stays at minus infinity
-        factors[row] = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(p.scale_log2), 1e-35f);
-      }
-    }
   }
   fence_proxy_async_smem();
   tc_fence_before();
@@ -234,10 +186,10 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
         if (x == 1) tc_commit(k_free + 8 * (i & 1));
       };
       fine = mbar_wait(k_full, 0);
-      tc_fence_after();
-      if (fine) {
-        scores(0, 0);
-        scores(1, 0);
+      for (int x = 0; x < 2 && fine; ++x) {
+        fine = mbar_wait(q_full + 8 * x, 0);
+        tc_fence_after();
+        if (fine) scores(x, 0);
       }
       for (int i = 0; i < tiles && fine; ++i) {
 #pragma unroll 1
@@ -436,7 +388,58 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     const int tok = kv4_div(at, p.by_group);
     const bool on = mine < live;
     const int limit = on ? len - run + tok + 1 : 0;
-    const float factor = factors[mine];
+    float factor;
+    {
+      // the row's queries: loads of whole sectors, stores of neighbouring 16-byte pieces
+      const T* src = static_cast<const T*>(p.q) + (q0 + tok) * p.q_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.q_head;
+      uint4 raw[HD / 8];
+      if (on && p.vec_q) {
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) raw[c] = on ? kv4_raw8(src + 8 * c, false) : make_uint4(0, 0, 0, 0);
+      }
+      float big = 0.0f;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        float y[8];
+        kv4_floats8<T>(raw[c], y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(y[i]));
+      }
+      const int e = big > 0.0f ? min(120, max(-120, static_cast<int>(__float_as_uint(big) >> 23) - 127)) : 0;
+      // a negative scale is taken into q, so that the largest score is the largest product
+      const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.scale_log2);
+      // never zero, so that a hidden score stays at minus infinity
+      factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(p.scale_log2), 1e-35f);
+      uint8_t* q = smem + x * Shape::kQ + row * 16;
+      uint32_t lead[2] = {0, 0}, rest[2] = {0, 0};
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 4 * g; c < 4 * g + 4; ++c) {
+          float y[8];
+          kv4_floats8<T>(raw[c], y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            y[i] *= down;
+            sum += y[i];
+          }
+          *reinterpret_cast<uint4*>(q + c * Shape::kLeadQ) =
+              make_uint4(pack_f16(y[0], y[4]), pack_f16(y[1], y[5]), pack_f16(y[2], y[6]), pack_f16(y[3], y[7]));
+        }
+        const __half hi = __float2half_rn(sum);
+        lead[g / 2] |= static_cast<uint32_t>(__half_as_ushort(hi)) << (16 * (g & 1));
+        rest[g / 2] |= static_cast<uint32_t>(__half_as_ushort(__float2half_rn(sum - __half2float(hi)))) << (16 * (g & 1));
+      }
+      *reinterpret_cast<uint4*>(q + HD / 8 * Shape::kLeadQ) = make_uint4(lead[0], lead[1], rest[0], rest[1]);
+      *reinterpret_cast<uint4*>(q + (HD / 8 + 1) * Shape::kLeadQ) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + 8 * x);
+    }
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;      // 32 tensor memory lanes a warp
     const uint32_t s_at = tmem + lanes + Shape::kColS + x * KT, o_at = tmem + lanes + Shape::kColO + x * Shape::kWide;
     float top = -INFINITY;                  // maximum in use, log2 units
