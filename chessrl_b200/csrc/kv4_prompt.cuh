@@ -39,7 +39,8 @@ struct Kv4PromptShape {
   static constexpr int kOffFlags = kOffV + 2 * kV;                 // 4 x 8 words of block flags
   static constexpr int kOffBad = kOffFlags + 4 * 8 * 4;            // 4 x kKeys bytes: groups of a key's value that are NaN
   static constexpr int kOffBars = (kOffBad + 4 * kKeys + 15) / 16 * 16;
-  static constexpr int kBytes = kOffBars + 20 * 8;
+  static constexpr int kBytes = kOffBars + 22 * 8;
+  static constexpr int kRow = HD * 2 + 16;                // a row of q or out on its way, padded onto distinct banks
   static constexpr int kThreads = 16 * 32;
   static constexpr int kColS = 0, kColO = 2 * kKeys;      // tensor memory columns: S_a, S_b, O_a, O_b
 };
@@ -128,8 +129,8 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
   const uint32_t bars = smem_u32(smem + Shape::kOffBars);
   // full / free per operand stage, then per row tile: scores there, weights there, output product done
   const uint32_t k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, p_full = bars + 80,
-                 o_done = bars + 96, p_half = bars + 112, q_full = bars + 128;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Shape::kOffBars + 144);
+                 o_done = bars + 96, p_half = bars + 112, q_full = bars + 128, q_raw = bars + 144;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Shape::kOffBars + 160);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
@@ -138,6 +139,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       mbar_init(v_full + 8 * s, NB);
       mbar_init(v_free + 8 * s, 1);
       mbar_init(q_full + 8 * s, 4);
+      mbar_init(q_raw + 8 * s, 1);
       mbar_init(s_full + 8 * s, 2);      // the products' commit and the issuing thread
       mbar_init(p_half + 8 * s, 4);
       mbar_init(p_full + 8 * s, 4);
@@ -390,16 +392,20 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     const int limit = on ? len - run + tok + 1 : 0;
     float factor;
     {
-      // the row's queries: loads of whole sectors, stores of neighbouring 16-byte pieces
+      // the row's queries, by one bulk copy into the place of the operands, from there into registers (16-byte loads from
+      // global memory by row took four times as long)
       const T* src = static_cast<const T*>(p.q) + (q0 + tok) * p.q_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.q_head;
+      uint8_t* place = smem + x * Shape::kQ + row * Shape::kRow;
       uint4 raw[HD / 8];
-      if (on && p.vec_q) {
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-      } else {
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) raw[c] = on ? kv4_raw8(src + 8 * c, false) : make_uint4(0, 0, 0, 0);
+      if (p.vec_q) {
+        if (row == 0) mbar_expect_tx(q_raw + 8 * x, max(0, min(live - x * 128, 128)) * HD * 2);
+        if (on) bulk_load(smem_u32(place), src, HD * 2, q_raw + 8 * x);
+        if (!mbar_wait(q_raw + 8 * x, 0)) fine = false;
       }
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+        raw[c] = !on ? make_uint4(0, 0, 0, 0) : p.vec_q ? *reinterpret_cast<const uint4*>(place + 16 * c) : kv4_raw8(src + 8 * c, false);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");      // the four warps of the row tile have read
       float big = 0.0f;
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c) {
@@ -521,6 +527,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
       tc_fence_after();
     }
     T* out = static_cast<T*>(p.out) + (q0 + tok) * p.o_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.o_head;
+    T* place = reinterpret_cast<T*>(smem + x * Shape::kQ + row * Shape::kRow);      // the queries' place: their products are through
     uint32_t cen[16];
     if (fine && tiles > 0) {
       tmem_ld_x16(o_at + HD, cen);
@@ -546,8 +553,14 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
         float z[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] = y[8 * h + j];
-        kv4_store8(out + c + 8 * h, p.vec_o, z);
+        kv4_store8(p.vec_o ? place + c + 8 * h : out + c + 8 * h, p.vec_o, z);
       }
+    }
+    if (p.vec_o && on) {      // the row leaves by one bulk copy
+      fence_proxy_async_smem();
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out), "r"(smem_u32(place)), "r"(HD * 2) : "memory");
+      bulk_commit();
+      bulk_wait_read0();
     }
   }
   if (!fine && lane == 0) kv4_report(p.status, kDevKv4Timeout);
