@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, __half2 s) {
 }
 
 template <typename T, int HD, int RW, int KW>
-__global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4AttentionParams p) {
+__global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kernel(const Kv4AttentionParams p) {
   using Shape = Kv4RowsShape<HD, RW, KW>;
   constexpr int G = HD / 32, DT = HD / 8, BB = kv4_block_bytes(HD), ROWS = 16 * RW, ST = Shape::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -51,6 +51,14 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   // which blocks of a stage's tile there are, left by the warp that copies them
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + Shape::kBytes - KW * ST * 4) + kw * ST;
 
+  // the first tiles' pages are asked for together with the sequence's length and its run of new tokens
+  const int first = rank * KW + kw, step = splits * KW;
+  const int32_t* pages_of = p.table.table + seq * p.table.stride;
+  const int lookers = p.whole_tiles ? 1 : 4;
+  uint32_t ahead[ST];
+#pragma unroll
+  for (int s = 0; s < ST; ++s)
+    ahead[s] = rw == 0 && lane < lookers ? kv4_block_of(p.table, pages_of, (first + s * step) * 4 + lane) : kNoBlock;
   int len = p.lengths[seq];
   const int64_t q0 = p.cu != nullptr ? p.cu[seq] : seq;
   int run = p.cu != nullptr ? p.cu[seq + 1] - p.cu[seq] : 1;
@@ -77,31 +85,31 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   mbar_fence_init();
   __syncthreads();
 
-  const int first = rank * KW + kw, step = splits * KW;
-  // lane b of a key group's first warp looks block b of a tile up (well before it is wanted) and copies it
-  const int32_t* pages_of = p.table.table + seq * p.table.stride;
+  // lane b of a key group's first warp looks block b of a tile up (well before it is wanted) and copies it; where pages
+  // hold whole tiles lane 0 does so for all
   const uint8_t* head_pages = p.pages + static_cast<size_t>(head) * p.table.blocks * BB;
-  auto look_up = [&](int tile) -> uint32_t {
-    if (lane >= min(4, blocks - tile * 4)) return kNoBlock;
-    const uint32_t at = kv4_block_of(p.table, pages_of, tile * 4 + lane);
-    if (at == kNoBlock) kv4_report(p.status, kDevKv4Table);
-    return at;
-  };
-  auto issue = [&](uint32_t at, int stage) {
-    const uint32_t there = __ballot_sync(0xffffffffu, at != kNoBlock);
+  auto issue = [&](uint32_t at, int tile, int stage) {
+    const int n = min(4, blocks - tile * 4);
+    if (lane < min(lookers, n)) {
+      if (at == kNoBlock) kv4_report(p.status, kDevKv4Table);
+    } else {
+      at = kNoBlock;
+    }
+    uint32_t there = __ballot_sync(0xffffffffu, at != kNoBlock);
+    const uint32_t to = smem_u32(ring + stage * Shape::kStage), bar = full + stage * 8;
+    if (p.whole_tiles) there = there != 0 ? (1u << n) - 1 : 0u;
     if (lane == 0) {
       held[stage] = there;
-      mbar_expect_tx(full + stage * 8, __popc(there) * BB);
+      mbar_expect_tx(bar, __popc(there) * BB);
+      if (p.whole_tiles && there != 0) bulk_load(to, head_pages + static_cast<size_t>(at) * BB, n * BB, bar);
     }
     __syncwarp();
-    if (at != kNoBlock)
-      bulk_load(smem_u32(ring + stage * Shape::kStage + lane * BB),
-                head_pages + static_cast<size_t>(at) * BB, BB, full + stage * 8);
+    if (!p.whole_tiles && at != kNoBlock) bulk_load(to + lane * BB, head_pages + static_cast<size_t>(at) * BB, BB, bar);
   };
   if (rw == 0)
 #pragma unroll
     for (int s = 0; s < ST; ++s)
-      if (first + s * step < tiles) issue(look_up(first + s * step), s);
+      if (first + s * step < tiles) issue(ahead[s], first + s * step, s);
 
   // queries as the A operand, rows r and r + 8 of this warp, scaled to [1, 2) by a power of two
   uint32_t qf[G][2][4], qsum[2] = {0, 0};     // [group][half of the group][register]; sums: rows r, r + 8
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
   bool fine = true;
   for (int tile = first; tile < tiles; tile += step) {
     const bool more = rw == 0 && tile + ST * step < tiles;
-    const uint32_t ahead = more ? look_up(tile + ST * step) : kNoBlock;
+    const uint32_t then = more && lane < lookers ? kv4_block_of(p.table, pages_of, (tile + ST * step) * 4 + lane) : kNoBlock;
     if (!mbar_wait(full + stage * 8, phase)) { fine = false; break; }
     const uint32_t there = held[stage];
     if (tile * 64 < see_any) {
@@ -336,7 +344,7 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
     if (lane == 0) mbar_arrive(empty + stage * 8);
     if (more) {
       if (!mbar_wait(empty + stage * 8, phase)) { fine = false; break; }
-      issue(ahead, stage);
+      issue(then, tile + ST * step, stage);
     }
     if (++stage == ST) {
       stage = 0;
@@ -348,6 +356,32 @@ __global__ void __launch_bounds__(RW * KW * 32) kv4_rows_kernel(const Kv4Attenti
     for (int s = 0; s < ST; ++s) mbar_wait(full + s * 8, s < stage ? phase ^ 1u : phase);
   }
 
+  if (KW == 1 && splits == 1) {      // nothing to join: from the registers
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+      const int at = row0 + rw * 16 + r + 8 * h, tok = kv4_div(at, p.by_group);
+      const float inv = sum[h] == 0.0f ? 0.0f : 1.0f / sum[h];      // a row that sees nothing is zero
+      T* out = static_cast<T*>(p.out) + (q0 + tok) * p.o_tok + static_cast<int64_t>(head * p.group + at - tok * p.group) * p.o_head + 2 * t;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float c = __shfl_sync(0xffffffffu, cen[2 * h + (g & 1)], (lane & ~3) + g / 2);
+        if (tok >= run) continue;
+#pragma unroll
+        for (int d = 4 * g; d < 4 * g + 4; ++d) {
+          T two[2] = {kv4_from_float<T>((acc[d][2 * h] + c) * inv), kv4_from_float<T>((acc[d][2 * h + 1] + c) * inv)};
+          if (p.pair_o) {
+            *reinterpret_cast<uint32_t*>(out + 8 * d) = *reinterpret_cast<const uint32_t*>(two);
+          } else {
+            out[8 * d] = two[0];
+            out[8 * d + 1] = two[1];
+          }
+        }
+      }
+    }
+    return;
+  }
   // join over the key groups, then over the cluster
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem) + warp * (Shape::kPart / 4);

@@ -196,9 +196,10 @@ int attend_few_by_rows(const Kv4AttentionParams& p, int64_t rows, int64_t max_ke
   if constexpr (HD > 32) return attend_few<T, HD, 0, WARPS>(p, max_keys, s);
 }
 template <typename T, int HD, int RW>
-int attend_rows(const Kv4AttentionParams& p, int64_t max_keys, cudaStream_t s) {
+int attend_rows(Kv4AttentionParams p, int64_t max_keys, cudaStream_t s) {
   using Shape = Kv4RowsShape<HD, RW, 4 / RW>;
   static KernelFacts facts[64];
+  p.whole_tiles = p.table.blocks % 4 == 0;
   return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, facts, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, p, max_keys, s);
 }
 template <typename T, int HD>
