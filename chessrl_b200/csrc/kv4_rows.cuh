@@ -174,8 +174,14 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
     constexpr bool MASKED = decltype(masked_tag)::value;
     const uint8_t* base = ring + stage * Shape::kStage;
     float sc[8][4];
+    // blocks of the tile that any of the warp's rows sees
+    const int seen = MASKED ? min(4, (see_any - tile * 64 + 15) / 16) : 4;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+      if (MASKED && j / 2 >= seen) {
+        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = -INFINITY;
+        continue;
+      }
       const uint8_t* blk = base + (j >> 1) * BB;
       const int key = kr + 8 * (j & 1);
       uint32_t w[G], m[G];
@@ -241,6 +247,7 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
       }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
+      if (MASKED && b >= seen) break;
       const uint8_t* blk = base + b * BB + 10 * HD;
       const uint32_t a0 = pack_f16(sc[2 * b][0], sc[2 * b][1]), a1 = pack_f16(sc[2 * b][2], sc[2 * b][3]);
       const uint32_t a2 = pack_f16(sc[2 * b + 1][0], sc[2 * b + 1][1]), a3 = pack_f16(sc[2 * b + 1][2], sc[2 * b + 1][3]);
@@ -250,23 +257,26 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
       if (MASKED) {
         // rows that no query sees may hold anything; a NaN that some rows see and others do not must not reach the
         // others through 0 * NaN in the product: it is taken out and given to the rows that see it
-        uint32_t bad[4];
-        bool any = false;
+        __half2 probe = __float2half2_rn(0.0f);      // 0 * m is NaN for a NaN or an infinity
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const bool gone = tile * 64 + b * 16 + t + 4 * k >= see_any || !((there >> b) & 1u);
-          bad[k] = 0;
 #pragma unroll
           for (int g = 0; g < G; ++g) {
             if (gone) m[k][g] = 0u;
-            if ((m[k][g] & 0x7c00u) == 0x7c00u || (m[k][g] & 0x7c000000u) == 0x7c000000u) {
-              bad[k] |= 1u << g;
-              m[k][g] = 0u;
-            }
+            probe = __hfma2(as_half2(m[k][g]), __float2half2_rn(0.0f), probe);
           }
-          any |= bad[k] != 0;
         }
-        if (__any_sync(0xffffffffu, any)) {
+        if (__any_sync(0xffffffffu, (as_word(probe) & 0x7fff7fffu) != 0)) {
+          uint32_t bad[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              if ((m[k][g] & 0x7c00u) == 0x7c00u || (m[k][g] & 0x7c000000u) == 0x7c000000u) {
+                bad[k] |= 1u << g;
+                m[k][g] = 0u;
+              }
           uint32_t lost[2] = {0, 0};
           for (int key = 0; key < 16; ++key) {
             const uint32_t mine = key / 4 == 0 ? bad[0] : key / 4 == 1 ? bad[1] : key / 4 == 2 ? bad[2] : bad[3];
