@@ -50,11 +50,11 @@ template <> __device__ __forceinline__ __nv_bfloat16 logit_from(float x) { retur
 
 // table entry: how often the token was said (low 20 bits), 1 + the number of its last bias entry (high 12)
 constexpr int kLogitsMaxHistory = (1 << 20) - 1, kLogitsMaxBiases = (1 << 12) - 2;
-constexpr int kLogitsThreads = 256;
+constexpr int kLogitsThreads = 256, kLogitsAhead = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads) adjust_logits_kernel(const LogitsParams p) {
-  extern __shared__ __align__(16) uint32_t table[];
+  extern __shared__ __align__(16) uint32_t room[];
   constexpr int VEC = 16 / sizeof(T);
   const int64_t row = blockIdx.x / p.tiles;
   const int tile = static_cast<int>(blockIdx.x - row * p.tiles);
@@ -63,8 +63,32 @@ __global__ void __launch_bounds__(kLogitsThreads) adjust_logits_kernel(const Log
   const T* in = static_cast<const T*>(p.in) + row * p.in_stride + v0;
   T* out = static_cast<T*>(p.out) + row * p.out_stride + v0;
   const float* values = p.bias_values + (p.biases > 0 ? row * p.value_stride : 0);
+  // 16-byte pieces from the first boundary on, single elements around them; a thread's pieces are under way while the
+  // table is made
+  const int lead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / static_cast<int>(sizeof(T));
+  const int head = p.same_phase ? min(lead, n) : n;
+  const int pieces = (n - head) / VEC;
+  uint32_t* table = room + ((4 - (head & 3)) & 3);      // a piece's entries start on a 16-byte boundary
+  uint4 ahead[kLogitsAhead];
+#pragma unroll
+  for (int u = 0; u < kLogitsAhead; ++u) {
+    const int q = threadIdx.x + u * kLogitsThreads;
+    ahead[u] = q < pieces ? *reinterpret_cast<const uint4*>(in + head + q * VEC) : make_uint4(0, 0, 0, 0);
+  }
+  const float rep = p.repetition != nullptr ? p.repetition[row] : 1.0f;
+  const float freq = p.frequency != nullptr ? p.frequency[row] : 0.0f;
+  const float pres = p.presence != nullptr ? p.presence[row] : 0.0f;
+  const uint8_t* bits = nullptr;
+  if (p.mask != nullptr) {
+    const int64_t m = p.mask_rows != nullptr ? p.mask_rows[row] : row;
+    if (m >= p.mask_count) {
+      if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kDevLogitsMaskRow));
+    } else if (m >= 0) {
+      bits = p.mask + m * p.mask_stride;
+    }
+  }
   if (marks) {
-    for (int i = threadIdx.x; i < n; i += kLogitsThreads) table[i] = 0;
+    for (int i = threadIdx.x; i < (n + 6) / 4; i += kLogitsThreads) reinterpret_cast<uint4*>(room)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const int32_t* ids = p.bias_ids + (p.biases > 0 ? row * p.bias_stride : 0);
     for (int i = threadIdx.x; i < p.biases; i += kLogitsThreads) {
@@ -81,42 +105,22 @@ __global__ void __launch_bounds__(kLogitsThreads) adjust_logits_kernel(const Log
     }
     __syncthreads();
   }
-  const float rep = p.repetition != nullptr ? p.repetition[row] : 1.0f;
-  const float freq = p.frequency != nullptr ? p.frequency[row] : 0.0f;
-  const float pres = p.presence != nullptr ? p.presence[row] : 0.0f;
-  const uint8_t* bits = nullptr;
-  if (p.mask != nullptr) {
-    const int64_t m = p.mask_rows != nullptr ? p.mask_rows[row] : row;
-    if (m >= p.mask_count) {
-      if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kDevLogitsMaskRow));
-    } else if (m >= 0) {
-      bits = p.mask + m * p.mask_stride;
-    }
-  }
-  auto one = [&](T x, int i, bool allowed) -> T {
+  const T masked = logit_from<T>(p.masked_value);
+  auto adjusted = [&](T x, uint32_t mark) -> T {
     float z = logit_to<T>(x);
-    if (marks) {
-      const uint32_t mark = table[i];
-      if (mark != 0) {
-        const uint32_t count = mark & 0xfffffu, last = mark >> 20;
-        if (count != 0) {
-          z = z > 0.0f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
-          z = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, static_cast<float>(count)), pres));
-        }
-        if (last != 0) z = __fadd_rn(z, values[last - 1]);
-      }
+    const uint32_t count = mark & 0xfffffu, last = mark >> 20;
+    if (count != 0) {
+      z = z > 0.0f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
+      z = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, static_cast<float>(count)), pres));
     }
-    return logit_from<T>(allowed ? z : p.masked_value);
+    if (last != 0) z = __fadd_rn(z, values[last - 1]);
+    return logit_from<T>(z);
   };
   auto allowed = [&](int i) { return bits == nullptr || ((bits[(v0 + i) >> 3] >> ((v0 + i) & 7)) & 1) != 0; };
-  // 16-byte pieces from the first boundary on, single elements around them
-  const int lead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / static_cast<int>(sizeof(T));
-  const int head = p.same_phase ? min(lead, n) : n;
-  const int pieces = (n - head) / VEC;
-  for (int q = threadIdx.x; q < pieces; q += kLogitsThreads) {
+  auto piece = [&](int q, const uint4& raw) {
     const int i = head + q * VEC;
     T x[VEC];
-    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(in + i);
+    *reinterpret_cast<uint4*>(x) = raw;
     uint32_t m = ~0u;
     if (bits != nullptr) {
       const int v = v0 + i, b = v >> 3;
@@ -124,14 +128,42 @@ __global__ void __launch_bounds__(kLogitsThreads) adjust_logits_kernel(const Log
       if ((v & 7) + VEC > 8) m |= static_cast<uint32_t>(bits[b + 1]) << 8;
       m >>= v & 7;
     }
+    if (marks) {
+      uint32_t mark[VEC], any = 0;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = one(x[j], i + j, (m >> j) & 1u);
+      for (int j = 0; j < VEC; j += 4) *reinterpret_cast<uint4*>(mark + j) = *reinterpret_cast<const uint4*>(table + i + j);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) any |= mark[j];
+      if (any != 0) {
+        // marked entries are few and most of them masked: one after the other rather than all eight alike
+        uint32_t left = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) left |= mark[j] != 0 ? 1u << j : 0u;
+        for (left &= m; left != 0; left &= left - 1) {
+          const int at = __ffs(left) - 1;
+          T y = x[0];
+#pragma unroll
+          for (int j = 1; j < VEC; ++j) y = at == j ? x[j] : y;
+          y = adjusted(y, table[i + at]);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) x[j] = at == j ? y : x[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = (m >> j) & 1u ? x[j] : masked;
     *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(x);
-  }
+  };
+#pragma unroll
+  for (int u = 0; u < kLogitsAhead; ++u)
+    if (threadIdx.x + u * kLogitsThreads < pieces) piece(threadIdx.x + u * kLogitsThreads, ahead[u]);
+  for (int q = threadIdx.x + kLogitsAhead * kLogitsThreads; q < pieces; q += kLogitsThreads)
+    piece(q, *reinterpret_cast<const uint4*>(in + head + q * VEC));
   const int tail = head + pieces * VEC, singles = head + n - tail;
   for (int q = threadIdx.x; q < singles; q += kLogitsThreads) {
     const int i = q < head ? q : tail + q - head;
-    out[i] = one(in[i], i, allowed(i));
+    const T x = in[i];
+    out[i] = !allowed(i) ? masked : marks && table[i] != 0 ? adjusted(x, table[i]) : x;
   }
 }
 

@@ -241,7 +241,7 @@ template <typename T>
 int logits_rows(const LogitsParams& p, cudaStream_t s) {
   const int64_t grid = p.rows * p.tiles;
   if (grid > INT32_MAX) return CRL_ERR_SHAPE;
-  adjust_logits_kernel<T><<<static_cast<unsigned>(grid), kLogitsThreads, p.tile * 4, s>>>(p);
+  adjust_logits_kernel<T><<<static_cast<unsigned>(grid), kLogitsThreads, (p.tile + 8) * 4, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? CRL_OK : CRL_ERR_CUDA;
 }
 
