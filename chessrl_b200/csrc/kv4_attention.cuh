@@ -155,13 +155,14 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) kv4_attention_kernel(c
     if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Table);
     len = static_cast<int>(room);
   }
+  const int before = len - max(run, 0);      // cache indices in front of the new tokens
   if (q0 < 0 || run < 0 || q0 + run > p.tokens || run > p.max_tokens) {
     if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Run);
     run = q0 < 0 || run < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(min(run, p.max_tokens)), max(p.tokens - q0, int64_t{0})));
   }
   const int live = run * p.group;                        // rows, at most eight
   if (live <= 0) return;                                 // the same for every CTA of the cluster
-  const int seen_most = max(0, len), seen_least = max(0, len - run + 1);
+  const int seen_most = max(0, min(len, before + run)), seen_least = max(0, before + 1);
   const int tiles = (seen_most + KEYS - 1) / KEYS, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
 
   if (lane < STAGES) mbar_init(bars + lane * 8, 1);
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) kv4_attention_kernel(c
     }
     // never zero, so that a hidden score stays at minus infinity
     const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + 24 + e) << 23) * fabsf(p.scale_log2), 1e-35f);
-    const int lim = on ? len - run + tok + 1 : 0;
+    const int lim = on ? before + tok + 1 : 0;
     // lane (r, t) needs columns 2t and 2t + 1: lanes 4 * (2t) and 4 * (2t + 1) hold them
 #pragma unroll
     for (int c = 0; c < C; ++c) {

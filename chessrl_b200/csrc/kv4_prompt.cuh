@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Table);
     len = static_cast<int>(room);
   }
+  const int before = len - max(run, 0);      // cache indices in front of the new tokens
   if (q0 < 0 || run < 0 || q0 + run > p.tokens || run > p.max_tokens) {
     if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Run);
     run = q0 < 0 || run < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(min(run, p.max_tokens)), max(p.tokens - q0, int64_t{0})));
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
   const int row0 = row_tile * 256, live = run * p.group - row0;     // rows of this CTA: min(live, 256)
   if (live <= 0) return;
   const int last_tok = kv4_div(row0 + min(live, 256) - 1, p.by_group);
-  const int seen_most = max(0, min(len, len - run + last_tok + 1));
+  const int seen_most = max(0, min(len, before + last_tok + 1));
   const int tiles = (seen_most + KT - 1) / KT;
 
   uint32_t* flags = reinterpret_cast<uint32_t*>(smem + Shape::kOffFlags);
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(Kv4PromptShape<HD>::kThreads, 1) kv4_prompt_ke
     const int x = warp >> 2, row = threadIdx.x & 127, mine = x * 128 + row, at = row0 + mine;
     const int tok = kv4_div(at, p.by_group);
     const bool on = mine < live;
-    const int limit = on ? len - run + tok + 1 : 0;
+    const int limit = on ? before + tok + 1 : 0;
     float factor;
     {
       // the row's queries, by one bulk copy into the place of the operands, from there into registers (16-byte loads from

@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
     if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Table);
     len = static_cast<int>(room);
   }
+  const int before = len - max(run, 0);      // cache indices in front of the new tokens
   if (q0 < 0 || run < 0 || q0 + run > p.tokens || run > p.max_tokens) {
     if (threadIdx.x == 0) kv4_report(p.status, kDevKv4Run);
     run = q0 < 0 || run < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(min(run, p.max_tokens)), max(p.tokens - q0, int64_t{0})));
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
   const int row0 = row_tile * ROWS, rows = run * p.group - row0;
   if (rows <= 0) return;      // the same for every CTA of the cluster
   const int last_tok = kv4_div(min(row0 + ROWS - 1, run * p.group - 1), p.by_group);
-  const int seen_most = max(0, min(len, len - run + last_tok + 1));
+  const int seen_most = max(0, min(len, before + last_tok + 1));
   const int tiles = (seen_most + 63) / 64, blocks = (seen_most + kKv4Block - 1) / kKv4Block;
 
   if (threadIdx.x < KW * ST) {
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
     const int e = big > 0.0f ? min(120, max(-120, static_cast<int>(__float_as_uint(big) >> 23) - 127)) : 0;
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
     factor[h] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * p.scale_log2;
-    limit[h] = live ? len - run + tok + 1 : 0;
+    limit[h] = live ? before + tok + 1 : 0;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float sum = 0.0f;
@@ -167,8 +168,8 @@ __global__ void __launch_bounds__(RW * KW * 32, HD == 128 ? 2 : 4) kv4_rows_kern
   const int kr = (r >> 1) + 4 * (r & 1);     // key of a half block that column r stands for
   // the tile's keys that every row of this warp sees, and those that any does
   const int warp_row = row0 + rw * 16, most_row = min(warp_row + 15, run * p.group - 1);
-  const int see_all = len - run + kv4_div(warp_row, p.by_group) + 1;
-  const int see_any = warp_row < run * p.group ? min(len, len - run + kv4_div(most_row, p.by_group) + 1) : 0;
+  const int see_all = before + kv4_div(warp_row, p.by_group) + 1;
+  const int see_any = warp_row < run * p.group ? min(len, before + kv4_div(most_row, p.by_group) + 1) : 0;
 
   auto consume = [&](auto masked_tag, int tile, int stage, uint32_t there) {
     constexpr bool MASKED = decltype(masked_tag)::value;

@@ -141,7 +141,7 @@ int facts_of(K* kernel, KernelFacts* all, int bytes, int threads, KernelFacts** 
 // The number of CTAs that share the keys of a (row tile, key head, sequence): the one that makes the waves of clusters
 // times the key tiles of the longest warp least (`fixed` tiles' worth of time goes to a CTA's start and join), for
 // sequences as long as the table allows.
-int split_keys(const KernelFacts& f, int64_t units, int64_t max_keys, int keys_at_once, int fixed) {
+int split_keys(const KernelFacts& f, int64_t units, int64_t max_keys, int keys_at_once, int fixed, int64_t* total = nullptr) {
   int best = 1;
   int64_t least = INT64_MAX;
   for (int n = 1; n <= kMaxSplits; ++n) {
@@ -156,6 +156,7 @@ int split_keys(const KernelFacts& f, int64_t units, int64_t max_keys, int keys_a
     }
     if (tiles <= 1) break;
   }
+  if (total != nullptr) *total = least;
   return best;
 }
 
@@ -196,11 +197,25 @@ int attend_few_by_rows(const Kv4AttentionParams& p, int64_t rows, int64_t max_ke
   if constexpr (HD > 32) return attend_few<T, HD, 0, WARPS>(p, max_keys, s);
 }
 template <typename T, int HD, int RW>
+KernelFacts rows_facts[64];
+// What the two kernels for many rows would take for sequences as long as the table allows, in hundreds of cycles: a CTA of
+// the first takes about 7000 per tile of 64 keys, one of the second 4400 per tile of 112 and 12000 to start and to end
+// (both measured at 4096-token prompts, head_dim 128). The first splits the keys over a cluster, the second does not.
+template <typename T, int HD>
+bool prompt_is_faster(const Kv4AttentionParams& p, int64_t rows, int sms, int64_t max_keys) {
+  using Shape = Kv4RowsShape<HD, 4, 1>;
+  KernelFacts* f = nullptr;
+  if (facts_of(kv4_rows_kernel<T, HD, 4, 1>, rows_facts<T, HD, 4>, Shape::kBytes, 128, &f) != CRL_OK) return false;
+  const int64_t pairs = static_cast<int64_t>(p.seqs) * p.kv_heads, ctas = pairs * ((rows + 255) / 256);
+  int64_t waves_tiles = 0;
+  split_keys(*f, pairs * ((rows + 63) / 64), max_keys, 64, 2, &waves_tiles);
+  return (ctas + sms - 1) / sms * ((max_keys + 111) / 112 * 44 + 120) < waves_tiles * 70;
+}
+template <typename T, int HD, int RW>
 int attend_rows(Kv4AttentionParams p, int64_t max_keys, cudaStream_t s) {
   using Shape = Kv4RowsShape<HD, RW, 4 / RW>;
-  static KernelFacts facts[64];
   p.whole_tiles = p.table.blocks % 4 == 0;
-  return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, facts, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, p, max_keys, s);
+  return attend_launch(kv4_rows_kernel<T, HD, RW, 4 / RW>, rows_facts<T, HD, RW>, Shape::kBytes, 128, 16 * RW, 4 / RW * 64, p, max_keys, s);
 }
 template <typename T, int HD>
 int attend_prompt(Kv4AttentionParams p, cudaStream_t s) {
@@ -232,7 +247,7 @@ struct Attend {
     }
     if (rows <= 16) return attend_rows<T, HD, 1>(p, max_keys, s);
     if (rows <= 32) return attend_rows<T, HD, 2>(p, max_keys, s);
-    if (rows > 128) return attend_prompt<T, HD>(p, s);
+    if (rows > 64 && prompt_is_faster<T, HD>(p, rows, sms, max_keys)) return attend_prompt<T, HD>(p, s);
     return attend_rows<T, HD, 4>(p, max_keys, s);
   }
 };

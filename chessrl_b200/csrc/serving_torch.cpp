@@ -231,6 +231,9 @@ Tensor kv4_attention(const Tensor& pages, const Tensor& q, const Tensor& table, 
     check_rows("out", *into, dev, heads, hd);
     check_type("out", *into, q.scalar_type());
     if (into->size(0) != tokens) refuse("out must have q's shape");
+    const int64_t st = into->stride(0), sh = into->stride(1);
+    const bool tokens_outside = st >= (heads - 1) * sh + hd && (heads == 1 || sh >= hd), heads_outside = sh >= (tokens - 1) * st + hd && (tokens == 1 || st >= hd);
+    if (tokens > 1 ? !tokens_outside && !(heads > 1 && heads_outside) : heads > 1 && sh < hd) refuse("the rows of out must not overlap");
     out = *into;
   } else {
     out = new_rows(q, tokens, heads, hd, q.scalar_type());
