@@ -201,6 +201,9 @@ KernelFacts rows_facts[64];
 // What the two kernels for many rows would take for sequences as long as the table allows, in hundreds of cycles: a CTA of
 // the first takes about 7000 per tile of 64 keys, one of the second 4400 per tile of 112 and 12000 to start and to end
 // (both measured at 4096-token prompts, head_dim 128). The first splits the keys over a cluster, the second does not.
+// First / second, measured: 32 new tokens at 60000, 12 heads on 1 of 64: 132 / 1176 us; 128-token prompts of 16 sequences,
+// 12 heads of 64: 14 / 26 us; 200 new tokens at 5000 in 4 sequences, 32 heads on 8 of 128: 471 / 140 us; a 2048-token
+// prompt of those heads: 375 / 84 us.
 template <typename T, int HD>
 bool prompt_is_faster(const Kv4AttentionParams& p, int64_t rows, int sms, int64_t max_keys) {
   using Shape = Kv4RowsShape<HD, 4, 1>;

@@ -161,6 +161,19 @@ def test_rows_behind_the_last_sequence_and_lost_indices(crl):
     assert int(status[0]) == 123
 
 
+def test_append_with_empty_sequences_and_shared_rows(crl):
+    """Sequences without new tokens among others, one row of keys for all heads (stride 0), more sequences than tokens."""
+    gen = torch.Generator().manual_seed(16)
+    new, before = [0, 3, 0, 0, 2, 0], [4, 0, 0, 9, 14, 1]
+    pages, table = pool(crl, [n + b for n, b in zip(new, before)], 16, 3, 32, gen)
+    cu = ints([0, 0, 3, 3, 3, 5, 5])
+    k = torch.randn(5, 1, 32, generator=gen).half().cuda().expand(5, 3, 32)
+    crl.kv4_append(pages, k, k, table, ints(before), cu_tokens=cu)
+    kh, vh = crl.kv4_read(pages, table, ints(before), 5, cu_tokens=cu)
+    want = spec.held_rows(k.cpu().float())[3].float().half()
+    assert torch.equal(kh.cpu(), want) and torch.equal(vh.cpu(), want)
+
+
 # ---- attention ------------------------------------------------------------------------------------------------------
 def attend_case(crl, dtype, hd, heads, kv, page, runs, seed=0, key_scale=1.0, value_scale=1.0, q_scale=1.0, scale=None, order=None):
     gen = torch.Generator().manual_seed(seed)
@@ -349,6 +362,105 @@ def test_attention_reports_what_it_skips(crl):
     status = ints([0])
     crl.kv4_attention(pages, q, table, ints([40, 20]), cu_tokens=ints([0, 1, 9]), max_tokens=8, out=out, status=status)
     assert int(status[0]) == 122
+
+
+def test_a_run_cut_short_keeps_its_positions(crl):
+    """max_tokens below a sequence's new tokens: the first max_tokens of them are computed at their own positions, the rest
+    of out is left alone, and the call reports it."""
+    gen = torch.Generator().manual_seed(12)
+    for n, most in ((6, 3), (40, 25), (500, 300)):
+        pages, table = filled(crl, [n + 30], 32, 2, 64, gen)
+        q = torch.randn(n, 4, 64, generator=gen).half().cuda()
+        whole = crl.kv4_attention(pages, q, table, ints([n + 30]), cu_tokens=ints([0, n]), max_tokens=n)
+        status, out = ints([0]), torch.full_like(q, 5.0)
+        crl.kv4_attention(pages, q, table, ints([n + 30]), cu_tokens=ints([0, n]), max_tokens=most, out=out, status=status)
+        assert int(status[0]) == 122 and (out[most:] == 5).all()
+        check_attention(out[:most], q[:most].contiguous(), pages, table, [(most, n + 30 - (n - most))])
+        assert (out[:most].float() - whole[:most].float()).abs().max() < 4e-3      # another kernel or tile, same rows
+
+
+@pytest.mark.parametrize("n", [1, 20, 300])
+def test_many_rows_with_odd_strides(crl, n):
+    """The other kernels with rows that are not 16-byte aligned, transposed heads, and a table inside a wider one."""
+    gen = torch.Generator().manual_seed(13)
+    lengths = [n + 40, n]
+    pages, table = filled(crl, lengths, 48, 2, 64, gen)
+    wide = torch.full((2, table.shape[1] + 5), -7, dtype=torch.int32, device="cuda")
+    wide[:, 2:2 + table.shape[1]] = table
+    total = 2 * n
+    q = torch.randn(total, 6 * 64 + 1, generator=gen).half().cuda()[:, 1:].unflatten(-1, (6, 64))
+    cu = ints([0, n, total])
+    out = torch.zeros(6, total, 64, dtype=F16, device="cuda").transpose(0, 1)
+    crl.kv4_attention(pages, q, wide[:, 2:2 + table.shape[1]], ints(lengths), cu_tokens=cu, max_tokens=n, out=out)
+    check_attention(out, q.contiguous(), pages, table, [(n, lengths[0]), (n, n)])
+    odd = torch.zeros(total, 6 * 64 + 1, dtype=F16, device="cuda")[:, 1:].unflatten(-1, (6, 64))
+    crl.kv4_attention(pages, q.contiguous(), table, ints(lengths), cu_tokens=cu, max_tokens=n, out=odd)
+    assert torch.equal(odd, out)
+    with pytest.raises(ValueError, match="overlap"):
+        crl.kv4_attention(pages, q, table, ints(lengths), cu_tokens=cu, max_tokens=n, out=out[:, :1].expand(total, 6, 64))
+
+
+def test_a_pool_beyond_four_gigabytes(crl):
+    """Offsets that pass 32 bits: pages at the end of a pool of 4.6 GB, and none of those whose offsets agree in 32 bits."""
+    size, kv, hd = 128, 8, 128
+    per_page = kv * size // 16 * 20 * hd
+    pages = crl.kv4_pages((1 << 32) // per_page + 2000, size, kv, hd)
+    gen = torch.Generator().manual_seed(14)
+    last = pages.shape[0] - 1
+    table = ints([last, last - 1500]).view(1, 2)
+    k, v = (torch.randn(200, kv, hd, generator=gen).half().cuda() for _ in range(2))
+    crl.kv4_append(pages, k, v, table, ints([0]), cu_tokens=ints([0, 200]))
+    kh, _ = crl.kv4_read(pages, table, ints([0]), 200, cu_tokens=ints([0, 200]))
+    assert torch.equal(kh.cpu(), spec.held_rows(k.cpu().float())[3].float().half())
+    assert not pages[:2000].any() and pages[last].any()
+    small, its = torch.stack([pages[last], pages[last - 1500]]), ints([0, 1]).view(1, 2)
+    for n in (1, 30, 200):
+        q = torch.randn(n, 8, hd, generator=gen).half().cuda()
+        far = crl.kv4_attention(pages, q, table, ints([200]), cu_tokens=ints([0, n]), max_tokens=n)
+        assert torch.equal(far, crl.kv4_attention(small, q, its, ints([200]), cu_tokens=ints([0, n]), max_tokens=n))
+
+
+def test_sequences_that_share_a_prefix(crl):
+    """Pages of a common prefix stand in several tables; each sequence goes on in its own."""
+    gen = torch.Generator().manual_seed(15)
+    pages, table = filled(crl, [32, 20, 20], 16, 2, 32, gen)
+    both = torch.stack([torch.cat([table[0], table[1]]), torch.cat([table[0], table[2]])]).contiguous()
+    runs = [(1, 52), (1, 47)]
+    q = torch.randn(2, 4, 32, generator=gen).half().cuda()
+    out = crl.kv4_attention(pages, q, both, ints([52, 47]))
+    check_attention(out, q, pages, both, runs)
+
+
+def test_first_calls_of_a_process_can_be_captured(crl):
+    """Nothing has to be called before a graph is captured."""
+    import subprocess
+    import sys
+    code = """
+import torch, chessrl_b200 as crl
+torch.zeros(1, device="cuda")
+pages = crl.kv4_pages(8, 16, 2, 64)
+table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+one, k = torch.tensor([3, 20], dtype=torch.int32, device="cuda"), torch.randn(2, 2, 64, device="cuda").half()
+rope, cu = crl.rope_table(64, 64), torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+big, cub = torch.randn(400, 4, 64, device="cuda").half(), torch.tensor([0, 200, 400], dtype=torch.int32, device="cuda")
+g = torch.cuda.CUDAGraph()
+def work():
+    q = crl.kv4_append(pages, k, k, table, one, q=k, rope=rope)
+    a = crl.kv4_attention(pages, q, table, one + 1)
+    b = crl.kv4_attention(pages, q.repeat(1, 5, 1), table, one + 1)
+    c = crl.kv4_attention(pages, big, table, one + 1, cu_tokens=cub, max_tokens=200)
+    return a, b, c, crl.adjust_logits(a.flatten(1), history=table), crl.kv4_read(pages, table, one, 2)[0]
+with torch.cuda.graph(g):
+    captured = work()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(captured, work()))
+print("captured")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+    assert "captured" in out.stdout, out.stderr[-2000:]
 
 
 # ---- logits ---------------------------------------------------------------------------------------------------------
