@@ -21,11 +21,14 @@
 // products then leaves each group's part in a column of its own, every lane applies one group's step and centre instead
 // of all, and the parts meet by one or two exchanges; likewise one set of P' columns serves all groups' output products.
 // COLS = 1 keeps to the even columns, so a lane has one row instead of two.
-// What is left is mostly the unpacking (88 of about 150 instructions per 16 tokens of 128 dims; 254 without).
+// What is left is mostly the unpacking (88 of about 150 instructions per 16 tokens of 128 dims; about 250 without).
 //
-// Bound by instruction issue above all (logical instructions run at half rate), memory next: 20 hd bytes per 16 cached
-// tokens and key head, brought in by bulk copies into a ring that belongs to the warp (no barrier among warps before the
-// join): one copy per tile where a page holds whole tiles, else one per block.
+// Each warp has a ring of bulk copies to itself (no barrier among warps before the join): one copy per tile where a page
+// holds whole tiles, else one per block. 128 registers, 16 warps per SM; 20 or 24 warps with fewer registers were no faster.
+// Measured: 256 sequences of up to 1024 tokens, 12 heads of 64: 50 us = 3.8 TB/s (the slope from 512 to 1024 tokens is
+// 5.5 TB/s; the rest is the start and the join of 3072 short clusters); 4 sequences of 131k tokens, 32 heads on 8 of 128:
+// 180 us = 3.0 TB/s, bound by issue (52 % of the slots; logical instructions run at half rate) on the SMs that have two
+// CTAs of a cluster of eight. Clusters of 9 to 16 pack worse onto the GPU's partitions (204 - 231 us).
 #pragma once
 #include <type_traits>
 

@@ -22,7 +22,14 @@
 // alike). Values are stored dim by dim along the keys: two keys' words give pairs of adjacent keys.
 //
 // A row's running maximum is only moved when it grows by more than 2^8 (P <= 256 stays well inside f16), so O is
-// rarely rescaled. Bound by: the exponentials (16 per cycle and SM: 128 x KT x 2 / 16 cycles per step) next to the products.
+// rarely rescaled.
+//
+// Measured: two prompts of up to 4096 tokens, 32 heads on 8 of 128, bf16: 384 us = 670 TFLOP/s, 41 % of the measured matrix
+// rate. A step of a row tile (112 keys) takes about 3500 cycles against 2230 of products for both tiles: the softmax
+// of one (2000) and the chain last weight -> output product -> scores (1500) follow one another, and two row tiles are
+// all that tensor memory holds at hd 128. The scores wait for the output product before them because they overwrite its weights.
+// Tried: taking turns with the exponentials (541 against 513 us then), reading the scores twice instead of keeping
+// them (503 against 406), issuing whichever row tile is ready first (501 against 390): none kept.
 #pragma once
 #include "kv4_rows.cuh"
 

