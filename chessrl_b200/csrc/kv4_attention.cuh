@@ -26,7 +26,7 @@
 // Each warp has a ring of bulk copies to itself (no barrier among warps before the join): one copy per tile where a page
 // holds whole tiles, else one per block. 128 registers, 16 warps per SM; 20 or 24 warps with fewer registers were no faster.
 // Measured: 256 sequences of up to 1024 tokens, 12 heads of 64: 50 us = 3.8 TB/s (the slope from 512 to 1024 tokens is
-// 5.5 TB/s; the rest is the start and the join of 3072 short clusters); 4 sequences of 131k tokens, 32 heads on 8 of 128:
+// 5.5 TB/s; the rest is the start and the join of 256 x 12 short clusters); 4 sequences of 131k tokens, 32 heads on 8 of 128:
 // 180 us = 3.0 TB/s, bound by issue (52 % of the slots; logical instructions run at half rate) on the SMs that have two
 // CTAs of a cluster of eight. Clusters of 9 to 16 pack worse onto the GPU's partitions (204 - 231 us).
 #pragma once

@@ -11,7 +11,7 @@
 // sixteen columns that hold c_g against the row's sum of q over group g (in two f16 parts), for the output one more
 // column block that collects sum p c_g. So only the weights p are rounded (f16), as a 16-bit cache would do as well.
 //
-// Bound by latency at the sizes it is for: 64-token prompts of 256 sequences, 12 heads of 64: 45 us (3072 CTAs of one tile
+// Bound by latency at the sizes it is for: 64-token prompts of 256 sequences, 12 heads of 64: 45 us (256 x 12 CTAs of one tile
 // each, four to an SM; issue slots 48 % used), 5-token runs of 33 sequences at 1000 tokens, 16 heads on 4 of 32: 11.4 us.
 // At 4096-token prompts it reaches 153 TFLOP/s where the kernel of kv4_prompt.cuh reaches 670.
 #pragma once

@@ -463,6 +463,32 @@ print("captured")
     assert "captured" in out.stdout, out.stderr[-2000:]
 
 
+@pytest.mark.parametrize("n", [1, 6, 30, 300])
+def test_keys_of_a_missing_page_are_left_out(crl, n):
+    """A page number outside the pool in the middle of a sequence: its tokens are as if they were not there, in every
+    kernel, and the call says so."""
+    gen = torch.Generator().manual_seed(18)
+    held = n + 200
+    for page in (16, 64):
+        pages, table = filled(crl, [held], page, 2, 64, gen)
+        broken = table.clone()
+        broken[0, 1] = pages.shape[0] + 3
+        q = torch.randn(n, 4, 64, generator=gen).half().cuda()
+        status = ints([0])
+        out = crl.kv4_attention(pages, q, broken, ints([held]), cu_tokens=ints([0, n]), max_tokens=n, status=status)
+        assert int(status[0]) == 121
+        for h in range(4):
+            k, v = spec.cache_rows(pages.cpu(), table[0].cpu(), held, h // 2)
+            keep = torch.ones(held, dtype=torch.bool)
+            keep[page:2 * page] = False
+            score = (q[:, h].cpu().double() @ k.T / 8.0)
+            seen = keep[None] & (torch.arange(held)[None] <= held - n + torch.arange(n)[:, None])
+            want = torch.softmax(score.masked_fill(~seen, -math.inf), 1) @ v
+            # as in check_attention
+            bound = v.abs().max() * (half_step(F16) * 2 + 2.0 ** -16 * (1 + score.abs().max())) + want.abs() * half_step(F16) + 1e-7
+            assert ((out[:, h].cpu().double() - want).abs() <= bound).all()
+
+
 # ---- logits ---------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
 @pytest.mark.parametrize("rows,vocab,said,biases", [(1, 1929, 40, 4), (5, 1929, 0, 0), (3, 7, 20, 9), (2, 1, 3, 1), (4, 8193, 300, 70),
