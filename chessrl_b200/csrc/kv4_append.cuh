@@ -6,8 +6,9 @@
 // stored as they are; value words are the transpose of 8 lanes x 8 nibbles, three exchanges away.
 //
 // Bound by instruction issue for prompts (the rotation is 13 instructions a value, see kv4_turn; the codes 6): 19k prompt
-// tokens of 32 + 2 x 8 heads of 128, half of each head rotated, appended and read back in 190 us (2.7 TB/s of the 6.5 that
-// a copy reaches; 40 registers and six CTAs per SM against 64 and four: 201). Single tokens are bound by the launch:
+// tokens of 32 + 2 x 8 heads of 128, half of each head rotated, appended and read back in 178 us (2.9 TB/s of the 6.5 that
+// a copy reaches; 201 with 64 registers and four CTAs per SM instead of 40 and six, 190 with half-rotated query rows like
+// all others). Single tokens are bound by the launch:
 // 4.6 us for one, 6.2 us for 256 sequences, append and read together.
 #pragma once
 #include "kv4.cuh"
@@ -70,6 +71,37 @@ __device__ __forceinline__ void kv4_rotate(const T* row, bool vec, const float2*
       x[i] = kv4_turn(x[i], cs.x, first ? o : -o, cs.y);
     }
   }
+}
+
+// A query row of which half is rotated: every lane takes two pairs and four of the dims that stay, where eight neighbouring
+// dims to a lane would have half of the lanes do the arithmetic (rows 16-byte aligned).
+template <typename T, int HD>
+__device__ __forceinline__ void kv4_rotate_half_row(const T* row, T* out, const float2* rope, bool interleaved, int part) {
+  constexpr int ROT = HD / 2, APART = ROT / 2;
+  const uint2 stay = *reinterpret_cast<const uint2*>(row + ROT + 4 * part);
+  const float2 c0 = rope[2 * part], c1 = rope[2 * part + 1];
+  T x[4];      // interleaved: a0 b0 a1 b1; halves: a0 a1 b0 b1
+  if (interleaved) {
+    *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(row + 4 * part);
+  } else {
+    *reinterpret_cast<uint32_t*>(x) = *reinterpret_cast<const uint32_t*>(row + 2 * part);
+    *reinterpret_cast<uint32_t*>(x + 2) = *reinterpret_cast<const uint32_t*>(row + APART + 2 * part);
+  }
+  const float a0 = kv4_to_float(x[0]), b0 = kv4_to_float(interleaved ? x[1] : x[2]);
+  const float a1 = kv4_to_float(interleaved ? x[2] : x[1]), b1 = kv4_to_float(x[3]);
+  const T y0 = kv4_from_float<T>(kv4_turn(a0, c0.x, b0, c0.y)), z0 = kv4_from_float<T>(kv4_turn(b0, c0.x, -a0, c0.y));
+  const T y1 = kv4_from_float<T>(kv4_turn(a1, c1.x, b1, c1.y)), z1 = kv4_from_float<T>(kv4_turn(b1, c1.x, -a1, c1.y));
+  x[0] = y0;
+  x[1] = interleaved ? z0 : y1;
+  x[2] = interleaved ? y1 : z0;
+  x[3] = z1;
+  if (interleaved) {
+    *reinterpret_cast<uint2*>(out + 4 * part) = *reinterpret_cast<const uint2*>(x);
+  } else {
+    *reinterpret_cast<uint32_t*>(out + 2 * part) = *reinterpret_cast<const uint32_t*>(x);
+    *reinterpret_cast<uint32_t*>(out + APART + 2 * part) = *reinterpret_cast<const uint32_t*>(x + 2);
+  }
+  *reinterpret_cast<uint2*>(out + ROT + 4 * part) = stay;
 }
 
 constexpr int kKv4CtaTokens = 8, kKv4Threads = 256;
@@ -160,9 +192,14 @@ __global__ void __launch_bounds__(kKv4Threads, 6) kv4_append_kernel(const Kv4App
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (live && is_q) {
       const T* row = static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head;
-      kv4_load8(row + part * 8, p.vec_q, x);
-      kv4_rotate(row, p.vec_q, w.rope, p.rot, p.interleaved, part, x);
-      kv4_store8(static_cast<T*>(p.q_out) + tok * p.o_tok + h * p.o_head + part * 8, p.vec_o, x);
+      T* out = static_cast<T*>(p.q_out) + tok * p.o_tok + h * p.o_head;
+      if (w.rope != nullptr && p.rot == HD / 2 && p.vec_q && p.vec_o) {
+        kv4_rotate_half_row<T, HD>(row, out, w.rope, p.interleaved, part);
+      } else {
+        kv4_load8(row + part * 8, p.vec_q, x);
+        kv4_rotate(row, p.vec_q, w.rope, p.rot, p.interleaved, part, x);
+        kv4_store8(out + part * 8, p.vec_o, x);
+      }
     }
     const bool ok = live && !is_q && w.block != kNoBlock;
     if (!__any_sync(0xffffffffu, ok)) continue;

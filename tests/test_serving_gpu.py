@@ -63,6 +63,9 @@ def filled(crl, lengths, page, kv, hd, gen, key_scale=1.0, value_scale=1.0):
     (32, 1, 7, 128, 32, True, [(130, 3)]),
     (128, 1, 2, 16, 6, False, [(3, 15), (2, 1)]),
     (64, 5, 5, 16, 10, True, [(20, 0)]),
+    (64, 2, 6, 16, 32, False, [(21, 5), (1, 0)]),
+    (32, 2, 4, 16, 16, True, [(9, 30), (14, 0)]),
+    (128, 1, 3, 32, 64, False, [(40, 7)]),
 ])
 def test_append_holds_the_defined_values(crl, dtype, hd, kv, heads, page, rot, interleaved, runs):
     gen = torch.Generator().manual_seed(hd + page + rot)
